@@ -3,12 +3,18 @@
 Python interface of ChenAo-Phys/fermix."""
 
 from .api import FermixDeviceError, FermixFallbackWarning, FermixTuneWarning, det, pf, slogdet, slogpf
+from .network import attention, attention_step, distance_buckets, relative_bias, residual_norm
 
 __all__ = [
     "slogdet",
     "slogpf",
     "det",
     "pf",
+    "distance_buckets",
+    "relative_bias",
+    "attention",
+    "attention_step",
+    "residual_norm",
     "FermixFallbackWarning",
     "FermixDeviceError",
     "FermixTuneWarning",

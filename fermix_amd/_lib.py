@@ -115,6 +115,68 @@ for _k in ("f64", "c64", "c128"):
     })
 
 
+# ------------------------------------------------- the network in front (include/fermix.h)
+
+# element types
+FX_F32, FX_F64, FX_BF16, FX_F16 = 0, 1, 2, 3
+FX_MAX_RADIUS = 2048
+FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE = 1, 2, 4
+FX_MAX_COLUMNS = 8192
+
+
+def _struct(name, layout):
+    """A ctypes structure from lines of "type: fields"."""
+    kinds = {"p": _p, "i64": _i64, "i32": _i32, "f32": ctypes.c_float}
+    fields = [(f, kinds[k]) for line in layout.strip().splitlines() for k, fs in [line.split(":")] for f in fs.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+FxAttention = _struct("FxAttention", """
+i64: batch
+i32: nq nk heads kv_heads dim dtype causal offset radius buckets
+f32: scale
+p: q k v
+i64: qb qn qh kb kn kh vb vn vh
+p: table map q_pos k_pos lengths q_lengths mask out stats grad_out grad_q grad_k grad_v grad_table
+""")
+
+FxAttentionStep = _struct("FxAttentionStep", """
+i64: batch
+i32: heads kv_heads dim dtype
+i64: pages
+i32: page_size max_pages radius buckets
+f32: scale
+p: q k v k_cache v_cache page_table lengths table map out
+""")
+
+FxResidualNorm = _struct("FxResidualNorm", """
+i64: samples rows
+i32: columns dtype wdtype flags
+f32: eps alpha
+p: x h gate
+i64: xs xr hs hr gs gr gc os or_
+p: post_weight post_bias scale pre_weight pre_bias y z stats
+p: grad_y grad_z grad_x grad_h grad_gate
+p: grad_post_weight grad_post_bias grad_scale grad_pre_weight grad_pre_bias
+""")
+
+for _n, _s in (("attention", FxAttention), ("residual_norm", FxResidualNorm)):
+    _sp = ctypes.POINTER(_s)
+    SIGNATURES[f"fx_{_n}_forward"] = (ctypes.c_int, [_sp, _p])
+    SIGNATURES[f"fx_{_n}_grad_workspace"] = (_sz, [_sp])
+    SIGNATURES[f"fx_{_n}_grad"] = (ctypes.c_int, [_sp, _p, _sz, _p])
+SIGNATURES.update({
+    "fx_relative_bias": (ctypes.c_int, [_p, _p, _i32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p]),
+    "fx_relative_bias_grad_workspace": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32]),
+    "fx_relative_bias_grad": (
+        ctypes.c_int,
+        [_p, _p, _i32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _sz, _p],
+    ),
+    "fx_attention_step_workspace": (_sz, [ctypes.POINTER(FxAttentionStep)]),
+    "fx_attention_step_run": (ctypes.c_int, [ctypes.POINTER(FxAttentionStep), _p, _sz, _p]),
+})
+
+
 class FermixLibraryError(RuntimeError):
     """The HIP library is missing, fails to load, or a call returned an error status."""
 

@@ -1,0 +1,366 @@
+// Attention with a relative position bias: what its forward and gradient kernels share.
+//
+// Products run on the 32 x 32 MFMA. Lane l = 32 h + c (h the half, c the column) of a wave holds
+//   A or B operand: row (column) c, the KS / 2 contraction indices KS s + (KS / 2) h .. of step s:
+//     16 bytes of a row, eight 16-bit or four float32 elements (four K = 2 products);
+//   accumulator: column c, rows 8 g + 4 h + r (g, r = 0..3) in register 4 g + r.
+// A product's accumulator, rounded to the type, is the B operand of the next product that contracts
+// over its rows, without a move between lanes: float32's indices agree, and for 16-bit types
+// the A operand takes the rows in the accumulator's order (16 s + 4 h + r, then 16 s + 8 + 4 h + r).
+// That A operand is a column read of a row-major tile: four float32 reads, or two transposing
+// 64-bit LDS reads (16 lanes read 4 rows of 16 columns, each gets one column).
+#pragma once
+#include "net.h"
+
+namespace fx {
+namespace net {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <class T>
+struct Mma;
+
+template <>
+struct Mma<float> {
+  static constexpr int KS = 8;
+  using frag = v4f;
+  static __device__ __forceinline__ v16f mma(frag a, frag b, v16f c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ frag columns(const float* tile, int stride, int row, int col, int lane) {
+    const float* p = tile + (row + 4 * (lane >> 5)) * stride + col + (lane & 31);
+    return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
+  }
+  static __device__ __forceinline__ frag from_acc(const v16f& x, int s) {
+    return frag{x[4 * s], x[4 * s + 1], x[4 * s + 2], x[4 * s + 3]};
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// Columns of four rows of a row-major 16-bit tile for 16 lanes at a time.
+__device__ __forceinline__ s16x4 read_columns4(const void* p) {
+  typedef __attribute__((address_space(3))) s16x4 lds_t;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(const s16x4*)p);
+}
+
+template <class T>
+struct Mma16 {
+  static constexpr int KS = 16;
+  using frag = vec_t<T, 8>;
+  static __device__ __forceinline__ frag columns(const T* tile, int stride, int row, int col, int lane) {
+    const T* p = tile + (row + 4 * (lane >> 5) + ((lane & 15) >> 2)) * stride + col + (lane & 16) + 4 * (lane & 3);
+    const s16x4 a = read_columns4(p), b = read_columns4(p + 8 * stride);
+    return __builtin_bit_cast(frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ frag from_acc(const v16f& x, int s) {
+    frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)x[8 * s + j];
+    return f;
+  }
+};
+template <>
+struct Mma<__bf16> : Mma16<__bf16> {
+  static __device__ __forceinline__ v16f mma(frag a, frag b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<_Float16> : Mma16<_Float16> {
+  static __device__ __forceinline__ v16f mma(frag a, frag b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// Row of register i of an accumulator in its half's lanes.
+__device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float F32_MAX = 3.402823466e38f;
+
+// A bias in the unit of the raw product q k (scores are c acc, c = scale log2 e): finite entries stay
+// finite, so that the type's lowest value weighs like any other and only -inf forbids.
+__device__ __forceinline__ float scaled_bias(float b, float inv_scale) {
+  const float x = b * inv_scale;
+  return isinf(b) || !(fabsf(x) > F32_MAX) ? x : copysignf(F32_MAX, b);
+}
+
+// exp2(c (s - m)) for a block of raw scores. One fma each while c m is small; past BASE_MAX (entries of the
+// table like the type's lowest value), where c m's own rounding would be a factor, and always for float32,
+// the difference is formed first.
+constexpr float BASE_MAX = 1024.0f;
+__device__ __forceinline__ void exp_block(v16f& s, float c, float m, float base, bool exact) {
+  if (exact) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f((s[i] - m) * c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));
+  }
+}
+
+constexpr int ATT_WAVES = 4, ATT_NT = 64 * ATT_WAVES;
+constexpr int ATT_TILE = 64;  // rows of a staged tile
+
+template <class T>
+constexpr int tile_stride(int dp) {
+  return dp + 16 / (int)sizeof(T);
+}
+
+// A tile of up to 64 rows of dim elements, through registers into LDS: fetch starts the loads, put
+// stores them. Rows at or past `rows`, and those that `live` refuses, become zero, so that nothing a
+// masked row holds enters a product; columns dim .. DP too.
+template <class T, int DP>
+struct TileLoad {
+  static constexpr int V = VEC16<T>, CHUNKS = DP / V, PER = ATT_TILE * CHUNKS / ATT_NT;
+  static_assert(PER >= 1 && PER * ATT_NT == ATT_TILE * CHUNKS, "whole turns");
+  vec_t<T, V> x[PER];
+
+  template <class L>
+  __device__ __forceinline__ void fetch(const T* base, int64_t row_stride, int rows, int dim, bool whole, L&& live) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = i * ATT_NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
+      x[i] = {};
+      if (r < rows && c < dim && live(r)) {
+        const T* p = base + r * row_stride + c;
+        if (whole) {
+          x[i] = *reinterpret_cast<const vec_t<T, V>*>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < dim) x[i][e] = p[e];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(T* tile) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = i * ATT_NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
+      *reinterpret_cast<vec_t<T, V>*>(tile + r * tile_stride<T>(DP) + c) = x[i];
+    }
+  }
+};
+
+// The operand of a wave's own rows straight from memory: row c of the lane, all steps.
+template <class T, int DP>
+struct RowFrags {
+  using M = Mma<T>;
+  static constexpr int STEPS = DP / M::KS, V = M::KS / 2;
+  typename M::frag f[STEPS];
+  __device__ __forceinline__ void load(const T* row, bool in, int dim, bool whole, int half) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int c = M::KS * s + V * half;
+      typename M::frag x = {};
+      if (in && c < dim) {
+        if (whole) {
+          x = *reinterpret_cast<const typename M::frag*>(row + c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < dim) x[e] = row[c + e];
+        }
+      }
+      f[s] = x;
+    }
+  }
+};
+
+// acc += (rows row0 .. row0 + 31 of the tile) x (the wave's rows): the tile's rows are the accumulator's.
+template <class T, int DP>
+__device__ __forceinline__ v16f row_product(const T* tile, int row0, const RowFrags<T, DP>& b, v16f acc, int lane) {
+  using M = Mma<T>;
+  const T* p = tile + (row0 + (lane & 31)) * tile_stride<T>(DP) + (M::KS / 2) * (lane >> 5);
+#pragma unroll
+  for (int s = 0; s < RowFrags<T, DP>::STEPS; ++s)
+    acc = M::mma(*reinterpret_cast<const typename M::frag*>(p + M::KS * s), b.f[s], acc);
+  return acc;
+}
+
+// acc[d] += (columns 32 d .. of the tile's rows row0 .. row0 + 31, transposed) x p, contracted over the rows.
+template <class T, int DP>
+__device__ __forceinline__ void column_product(const T* tile, int row0, const v16f& p, v16f (&acc)[DP / 32], int lane) {
+  using M = Mma<T>;
+#pragma unroll
+  for (int s = 0; s < 32 / M::KS; ++s) {
+    const typename M::frag b = M::from_acc(p, s);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+      acc[d] = M::mma(M::columns(tile, tile_stride<T>(DP), row0 + M::KS * s, 32 * d, lane), b, acc[d]);
+  }
+}
+
+// Maximum and sum of the lane's value and that of the lane 32 away.
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// A transposed accumulator (rows: 32 d + .. columns of the result; column: the lane's row) times f, as
+// rows of memory.
+template <class T, int DP>
+__device__ __forceinline__ void store_rows(T* row, const v16f (&acc)[DP / 32], float f, int dim, bool whole, int half) {
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * half;
+      vec_t<T, 4> x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = (T)(acc[d][4 * g + r] * f);
+      if (whole) {
+        if (c < dim) *reinterpret_cast<vec_t<T, 4>*>(row + c) = x;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (c + r < dim) row[c + r] = x[r];
+      }
+    }
+}
+
+// Bias of one head. Two forms:
+//  - positions that count up (GEN = false): the bias depends on key - query alone, so LDS holds it laid
+//    out over the distances -(R + 64) .. R + 64, saturated past R. A lane clamps once a tile, and
+//    the tile's values follow at constant offsets; a tile that lies past R as a whole has one value.
+//  - positions from memory (GEN = true): each pair's distance is clamped and looked up, map then table.
+struct BiasView {
+  float* lut;           // GEN: table [buckets]; else [2 R + 129] over distances
+  unsigned char* map;   // GEN: [2 R + 1]; else [2 R + 129] buckets over distances
+  int radius;
+};
+__device__ __host__ constexpr int bias_entries(bool gen, int radius) { return gen ? 2 * radius + 1 : 2 * radius + 129; }
+
+// Fills the view; `head` of the table (NULL: no bias). All threads of the workgroup; a barrier follows.
+template <bool GEN>
+__device__ __forceinline__ void fill_bias(const fx_attention& p, int head, const BiasView& b, float inv_scale) {
+  const int n = bias_entries(GEN, b.radius);
+  for (int i = threadIdx.x; i < n; i += ATT_NT) {
+    const int d = GEN ? i : max(0, min(2 * b.radius, i - 64));
+    const int t = p.table ? min((int)p.map[d], p.buckets - 1) : 0;
+    b.map[i] = (unsigned char)t;
+    if constexpr (!GEN) b.lut[i] = p.table ? scaled_bias(p.table[(int64_t)t * p.heads + head], inv_scale) : 0.0f;
+  }
+  if constexpr (GEN)
+    for (int i = threadIdx.x; i < p.buckets; i += ATT_NT)
+      b.lut[i] = p.table ? scaled_bias(p.table[(int64_t)i * p.heads + head], inv_scale) : 0.0f;
+}
+
+// A workgroup's place: items are laid out so that those of one kv head follow each other, and each of
+// the eight XCDs (workgroups go to them in turn) gets a contiguous part, whose K and V then stay
+// in its L2.
+__device__ __forceinline__ int64_t xcd_item(int64_t block, int64_t total) {
+  const int64_t per = total / 8, rest = total % 8, x = block % 8;
+  return x * per + (x < rest ? x : rest) + block / 8;
+}
+
+struct AttArgs {
+  fx_attention p;
+  int whole;   // rows are whole 16-byte vectors
+  int whole4;  // result rows are whole vectors of four elements
+  float c;     // scale log2(e)
+  float inv_scale;
+  int tiles;   // items of a head
+  int64_t items;
+  float* delta;  // gradient: [batch][heads][nq] sum_d out grad_out
+  float* part;   // gradient: bucket sums [head][batch * tiles][buckets]
+};
+
+// An item's place: sample, head and tile. Within a head the last tile comes first (with causal it has the
+// most keys), the heads that share K and V follow each other.
+struct Place {
+  int64_t b;
+  int h, tile;
+  __device__ __forceinline__ Place(int64_t item, int heads, int tiles) {
+    const int64_t bh = item / tiles;
+    tile = tiles - 1 - (int)(item - bh * tiles);
+    b = bh / heads;
+    h = (int)(bh - b * heads);
+  }
+};
+
+// What is left of a tile of keys: bit j of `ok` (GEN: mask), and a position for each key (GEN).
+struct KeyView {
+  int* pos;                // [64]
+  unsigned long long* ok;  // [1]
+};
+// By one wave, lane j for key k0 + j; a barrier follows.
+__device__ __forceinline__ void fill_keys(const fx_attention& p, int64_t b, int k0, int len, const KeyView& kv,
+                                          int lane) {
+  const int j = k0 + lane;
+  const bool in = j < len;
+  const bool ok = in && (!p.mask || p.mask[b * p.nk + j]);
+  kv.pos[lane] = !in ? 0 : p.k_pos ? p.k_pos[b * p.nk + j] : j;
+  const unsigned long long m = __ballot(ok);
+  if (lane == 0) *kv.ok = m;
+}
+
+// Whether a block of `rows` x `cols` pairs whose first distance (first key - first query) is d lies past the
+// radius as a whole: 1 above, -1 below, 0 neither. Distances run d - (queries - 1) .. d + (keys - 1).
+__device__ __forceinline__ int far_side(int d, int keys, int queries, int radius) {
+  return d - (queries - 1) >= radius ? 1 : d + (keys - 1) <= -radius ? -1 : 0;
+}
+
+// Start of a score block of 32 keys (rows k0 + 32 kb + ..) for the lane's query: the bias.
+template <bool GEN>
+__device__ __forceinline__ v16f bias_block(const fx_attention& p, const BiasView& bv, const KeyView& kv, int kb,
+                                           int k0, int qpos, int half, int far) {
+  v16f x;
+  if (!GEN && far) {
+    const float v = bv.lut[far > 0 ? 2 * bv.radius + 128 : 0];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = v;
+  } else if constexpr (GEN) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int4 kp = *reinterpret_cast<const int4*>(kv.pos + 32 * kb + 8 * g + 4 * half);
+      const int k[4] = {kp.x, kp.y, kp.z, kp.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = __builtin_elementwise_sub_sat(k[r], qpos);
+        x[4 * g + r] = bv.lut[bv.map[max(-bv.radius, min(bv.radius, d)) + bv.radius]];
+      }
+    }
+  } else {
+    const int d = max(-(bv.radius + 64), min(bv.radius, k0 - qpos));
+    const float* l = bv.lut + d + bv.radius + 64 + 32 * kb + 4 * half;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = l[acc_row(i)];
+  }
+  return x;
+}
+
+int launch_bucket_join(const float* part, int64_t n, int buckets, int heads, float* out, hipStream_t s);
+
+bool attention_sizes_ok(const fx_attention* p);
+bool attention_pointers_ok(const fx_attention& p);
+AttArgs attention_args(const fx_attention& p);
+
+// f(type, padded dim, positions or mask from memory)
+template <class F>
+int attention_shape(const fx_attention& p, F&& f) {
+  return with_type<false>(p.dtype, [&](auto t) {
+    auto by_gen = [&](auto dp) {
+      if (p.q_pos || p.mask)
+        f(t, dp, ic<1>{});
+      else
+        f(t, dp, ic<0>{});
+      return launched();
+    };
+    if (p.dim <= 32) return by_gen(ic<32>{});
+    if (p.dim <= 64) return by_gen(ic<64>{});
+    return by_gen(ic<128>{});
+  });
+}
+
+}  // namespace net
+}  // namespace fx

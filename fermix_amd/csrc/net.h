@@ -1,0 +1,69 @@
+// Shared by the kernels of the network in front of the determinants (relative position bias,
+// attention, its step over a paged cache, residual norms): element types, vector loads, wave
+// sums, distance buckets.
+#pragma once
+#include "common.h"
+#include "fermix_internal.h"
+
+namespace fx {
+namespace net {
+
+template <class T, int V>
+using vec_t = T __attribute__((ext_vector_type(V)));
+
+template <class T>
+__device__ __forceinline__ float to_f32(T x) {
+  return (float)x;
+}
+
+// Elements of a 16-byte vector.
+template <class T>
+constexpr int VEC16 = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ float shfl_xor(float x, int m) { return __shfl_xor(x, m, 64); }
+
+// Sum over the aligned group of W lanes (W a power of two up to 64); every lane gets it.
+template <int W>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int m = W / 2; m; m >>= 1) x += shfl_xor(x, m);
+  return x;
+}
+
+// Distance buckets: map[clamp(d, -radius, radius) + radius], clamped to the table's last row. The
+// distance saturates, so positions of any int32 value are in order.
+__device__ __forceinline__ int distance_bucket(const unsigned char* map, int radius, int buckets, int kpos, int qpos) {
+  const int d = __builtin_elementwise_sub_sat(kpos, qpos);
+  const int at = max(-radius, min(radius, d)) + radius;
+  return min((int)map[at], buckets - 1);
+}
+
+inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline int launched() { return hipGetLastError() == hipSuccess ? FX_OK : FX_ERR_LAUNCH; }
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline size_t dtype_size(int32_t dtype) {
+  switch (dtype) {
+    case FX_F32: return 4;
+    case FX_F64: return 8;
+    case FX_BF16:
+    case FX_F16: return 2;
+    default: return 0;
+  }
+}
+
+// f(T{}) with the element type of dtype; FX_ERR_UNSUPPORTED for another.
+template <bool F64, class F>
+inline int with_type(int32_t dtype, F&& f) {
+  switch (dtype) {
+    case FX_F32: return f(float{});
+    case FX_BF16: return f(__bf16{});
+    case FX_F16: return f(_Float16{});
+    case FX_F64:
+      if constexpr (F64) return f(double{});
+      return FX_ERR_UNSUPPORTED;
+    default: return FX_ERR_INVALID_ARGUMENT;
+  }
+}
+
+}  // namespace net
+}  // namespace fx

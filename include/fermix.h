@@ -461,6 +461,142 @@ size_t fx_det_parts_c128_workspace(int64_t batch, int32_t n);
 int fx_det_parts_c128(const double* a, int64_t batch, int32_t n, double* sign, double* logabs, double* adj_t,
                       void* workspace, size_t workspace_bytes, fx_stream_t stream);
 
+/* ---------------------------------------------------------------- the network in front
+ * Operators of the network whose output is the orbital or pairing matrix; no counterpart in
+ * the reference. Element types (dtype): */
+#define FX_F32 0
+#define FX_F64 1
+#define FX_BF16 2
+#define FX_F16 3
+
+/* Learned relative position bias by distance buckets.
+ *   out[b][h][i][j] = table[bucket(k_pos[b][j] - q_pos[b][i])][h],
+ *   bucket(d) = min(map[clamp(d, -radius, radius) + radius], buckets - 1),
+ * table (buckets, heads), out (batch, heads, nq, nk), both of dtype (any of the four),
+ * contiguous; map 2 radius + 1 bytes, 0 <= radius <= FX_MAX_RADIUS; 1 <= buckets <= 256;
+ * q_pos (batch, nq) and k_pos (batch, nk) any int32 (the distance saturates). Pointers are
+ * aligned to their element. fx_relative_bias_grad: grad_table (buckets, heads) of dtype, the
+ * sum of grad_out over the pairs of each bucket, in float32 (float64 for float64), in an
+ * order that depends on the sizes alone. */
+#define FX_MAX_RADIUS 2048
+int fx_relative_bias(const void* table, const uint8_t* map, int32_t radius, int32_t buckets, const int32_t* q_pos,
+                     const int32_t* k_pos, int64_t batch, int32_t heads, int32_t nq, int32_t nk, int32_t dtype,
+                     void* out, fx_stream_t stream);
+size_t fx_relative_bias_grad_workspace(int32_t buckets, int64_t batch, int32_t heads, int32_t nq, int32_t nk,
+                                       int32_t dtype);
+int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radius, int32_t buckets,
+                          const int32_t* q_pos, const int32_t* k_pos, int64_t batch, int32_t heads, int32_t nq,
+                          int32_t nk, int32_t dtype, void* grad_table, void* workspace, size_t workspace_bytes,
+                          fx_stream_t stream);
+
+/* Attention with the relative position bias, for prompts and training.
+ *   S = scale q k^T + table[bucket(k_pos - q_pos)],  P = softmax of S over the keys that are
+ *   left,  out = P v;  a query that no key is left for gets 0.
+ * q, out: (batch, nq, heads, dim), k, v: (batch, nk, kv_heads, dim), heads a multiple of kv_heads
+ * (head h reads kv head h / (heads / kv_heads)), 1 <= dim <= 128, dtype FX_F32, FX_BF16 or
+ * FX_F16; own strides in elements for batch, token and head, dim contiguous. Scores, softmax
+ * and sums are float32; for the 16-bit types P (and dS) are rounded to dtype for the products.
+ * Keys: index j < lengths[b] (NULL: nk), mask[b][j] != 0 (NULL: all; mask (batch, nk) bytes) and,
+ * with causal, j <= offset + i. What is masked by lengths or mask may hold anything; a
+ * value that causal alone masks has to be finite. Queries i >= q_lengths[b] (NULL: nq) get 0
+ * and no gradient. Positions: q_pos (batch, nq), k_pos (batch, nk) together, or NULL: offset + i
+ * and j. table (buckets, heads) float32 or NULL (no bias), map and radius as above, buckets <= FX_MAX_ATTENTION_BUCKETS;
+ * its entries may be -inf, and entries of float32's lowest value weigh like any other.
+ *
+ * fx_attention_forward: out and, if given, stats (batch, heads, nq, 2): the largest S / scale and log2
+ * of the sum of exp(S - its maximum); 0 and +inf where there is no key.
+ * fx_attention_grad: grad_q, grad_k, grad_v (strides of their own: those of q, k, v in packed
+ * tensors) and grad_table (buckets, heads) float32 (NULL to skip) from grad_out (packed), out
+ * (packed) and stats. Deterministic: sums are in an order that depends on sizes alone. */
+#define FX_MAX_ATTENTION_BUCKETS 64
+typedef struct fx_attention {
+  int64_t batch;
+  int32_t nq, nk, heads, kv_heads, dim, dtype;
+  int32_t causal, offset, radius, buckets;
+  float scale; /* finite, > 0 */
+  const void *q, *k, *v;
+  int64_t qb, qn, qh, kb, kn, kh, vb, vn, vh;
+  const float* table;
+  const uint8_t* map;
+  const int32_t *q_pos, *k_pos, *lengths, *q_lengths;
+  const uint8_t* mask;
+  void* out;
+  float* stats;
+  const void* grad_out;
+  void *grad_q, *grad_k, *grad_v;
+  float* grad_table;
+} fx_attention;
+int fx_attention_forward(const fx_attention* p, fx_stream_t stream);
+size_t fx_attention_grad_workspace(const fx_attention* p);
+int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_bytes, fx_stream_t stream);
+
+/* One token of each sample over a paged cache. The cache holds pages of page_size tokens, k_cache
+ * and v_cache (pages, page_size, kv_heads, dim) packed; token t of sample b is in page
+ * page_table[b][t / page_size] at t % page_size (page_table (batch, max_pages)). With k and v
+ * (batch, kv_heads, dim): they are stored as token lengths[b], and the query, at that position,
+ * attends to tokens 0 .. lengths[b]; lengths[b] < 0 leaves a sample out. Without them the query
+ * is at lengths[b] - 1 and attends to tokens 0 .. lengths[b] - 1. A sample with no token gets 0;
+ * one whose tokens pass its table, or whose table names a page outside the cache, gets NaN and
+ * stores nothing there. q, out (batch, heads, dim) packed. Types, heads, table, map as for
+ * fx_attention. With several parts of the tokens at work (splits > 1 of the plan) the parts' sums
+ * go through the workspace. Two samples must not name the same page for the token that they store. */
+typedef struct fx_attention_step {
+  int64_t batch;
+  int32_t heads, kv_heads, dim, dtype;
+  int64_t pages;
+  int32_t page_size, max_pages;
+  int32_t radius, buckets;
+  float scale;
+  const void *q, *k, *v;
+  void *k_cache, *v_cache;
+  const int32_t *page_table, *lengths;
+  const float* table;
+  const uint8_t* map;
+  void* out;
+} fx_attention_step;
+size_t fx_attention_step_workspace(const fx_attention_step* p);
+int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t workspace_bytes, fx_stream_t stream);
+
+/* The norms around a residual block with its gate and residual scale, rows of C elements:
+ *   a = norm(h) post_weight + post_bias,  y = x + alpha scale gate a,
+ *   z = norm(y) pre_weight + pre_bias,
+ * norm(t) = t / sqrt(mean(t^2) + eps) (RMS) or the same of t - mean(t) (FX_NORM_LAYER). Without
+ * FX_NORM_POST a = h; without FX_NORM_PRE there is no z. Sums and statistics are float32; z is
+ * formed from y before y is rounded.
+ *
+ * The rows are seen as samples x rows: element c of row r of sample s is at s ss + r sr + c of
+ * x, h (own strides) and y, z, and of the gradients and cotangents (one further pair of strides,
+ * os / or_); the gate's at s gs + r gr + c gc (gc 0 or 1; zero strides where it is
+ * broadcast). x, h, gate, y, z, cotangents and their gradients have dtype (FX_F32, FX_BF16,
+ * FX_F16); weights, biases and scale (columns), each optional (NULL: 1 or 0), have wdtype,
+ * which is dtype or FX_F32. stats: 4 floats a row (mean and reciprocal deviation of h, then of
+ * y), written by the forward if given, read by the gradient. 1 <= columns <= FX_MAX_COLUMNS. */
+#define FX_NORM_LAYER 1
+#define FX_NORM_POST 2
+#define FX_NORM_PRE 4
+#define FX_MAX_COLUMNS 8192
+typedef struct fx_residual_norm {
+  int64_t samples, rows; /* rows of each sample */
+  int32_t columns;
+  int32_t dtype, wdtype;
+  int32_t flags; /* FX_NORM_* */
+  float eps, alpha;
+  const void *x, *h, *gate;
+  int64_t xs, xr, hs, hr, gs, gr, gc, os, or_;
+  const void *post_weight, *post_bias, *scale, *pre_weight, *pre_bias;
+  void *y, *z; /* forward */
+  float* stats;
+  /* gradient: cotangents (either may be NULL: zero) and results; grad_gate (a gate given) has
+   * the gate's broadcast shape: samples x rows x columns, 1 wherever its stride is zero, packed.
+   * The five column gradients (columns, of wdtype) may each be NULL. */
+  const void *grad_y, *grad_z;
+  void *grad_x, *grad_h, *grad_gate;
+  void *grad_post_weight, *grad_post_bias, *grad_scale, *grad_pre_weight, *grad_pre_bias;
+} fx_residual_norm;
+int fx_residual_norm_forward(const fx_residual_norm* p, fx_stream_t stream);
+size_t fx_residual_norm_grad_workspace(const fx_residual_norm* p);
+int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t workspace_bytes, fx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
