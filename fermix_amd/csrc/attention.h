@@ -326,8 +326,7 @@ __device__ __forceinline__ v16f bias_block(const fx_attention& p, const BiasView
       const int k[4] = {kp.x, kp.y, kp.z, kp.w};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = __builtin_elementwise_sub_sat(k[r], qpos);
-        x[4 * g + r] = bv.lut[bv.map[max(-bv.radius, min(bv.radius, d)) + bv.radius]];
+        x[4 * g + r] = bv.lut[distance_bucket(bv.map, bv.radius, k[r], qpos)];
       }
     }
   } else {

@@ -37,21 +37,14 @@ struct Sums {
 };
 __device__ __forceinline__ unsigned fixed_weight(float p) { return (unsigned)(p * 0x1p30f); }
 
-template <bool WEIGHTS>
-__device__ __forceinline__ void add_to(const Sums& sums, int bucket, float ds, float p) {
-  unsafeAtomicAdd(sums.ds + 64 * bucket, ds);
-  if (WEIGHTS) atomicAdd(sums.weight + 32 * bucket, fixed_weight(p));
-}
-
 // Adds a block's dS and P (rows: keys; column: the lane's query).
 template <bool GEN, bool WEIGHTS>
 __device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv, Sums& sums, const v16f& ds,
                                            const v16f& w, int kb, int k0, int qpos, int half, int far) {
-  float total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) total += ds[i];
-  sums.all += total;
   if (!GEN && far) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) total += ds[i];
     sums.far_ds[far > 0] += total;
     if (WEIGHTS) {
 #pragma unroll
@@ -59,6 +52,8 @@ __device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv
     }
     return;
   }
+  // all lookups before the first add: the compiler keeps a read that follows one behind it
+  int t[16];
   if constexpr (GEN) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -66,20 +61,27 @@ __device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv
       const int k[4] = {kp.x, kp.y, kp.z, kp.w};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = __builtin_elementwise_sub_sat(k[r], qpos);
-        add_to<WEIGHTS>(sums, bv.map[max(-bv.radius, min(bv.radius, d)) + bv.radius], ds[4 * g + r], w[4 * g + r]);
+        t[4 * g + r] = distance_bucket(bv.map, bv.radius, k[r], qpos);
       }
     }
   } else {
     const int d = max(-(bv.radius + 64), min(bv.radius, k0 - qpos));
     const unsigned char* l = bv.map + d + bv.radius + 64 + 32 * kb + 4 * half;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) add_to<WEIGHTS>(sums, l[acc_row(i)], ds[i], w[i]);
+    for (int i = 0; i < 16; ++i) t[i] = l[acc_row(i)];
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    add_pair(sums.ds, t[i], ds[i], t[i + 1], ds[i + 1]);
+    if (WEIGHTS) {
+      atomicAdd(sums.weight + 32 * t[i], fixed_weight(w[i]));
+      atomicAdd(sums.weight + 32 * t[i + 1], fixed_weight(w[i + 1]));
+    }
   }
 }
 
 template <class T, int DP, bool GEN>
-__global__ __launch_bounds__(ATT_NT, 1) void attention_dq_kernel(const AttArgs a) {
+__global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void attention_dq_kernel(const AttArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   using M = Mma<T>;
   const fx_attention& p = a.p;
@@ -132,7 +134,6 @@ __global__ __launch_bounds__(ATT_NT, 1) void attention_dq_kernel(const AttArgs a
       for (int e = 0; e < M::KS / 2; ++e) delta += (float)o.f[s][e] * (float)g.f[s][e];
     delta = half_sum(delta);
   }
-  if (qi < p.nq && half == 0) a.delta[stat] = delta;
   const float2 ml = in ? reinterpret_cast<const float2*>(p.stats)[stat] : make_float2(0.0f, INFINITY);
   const float base = ml.x * a.c + ml.y;
   const bool exact = sizeof(T) == 4 || __any(fabsf(ml.x * a.c) > BASE_MAX);
@@ -184,26 +185,35 @@ __global__ __launch_bounds__(ATT_NT, 1) void attention_dq_kernel(const AttArgs a
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - delta);
+      if (WEIGHTS) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums.all += dp[i];
+      }
       if (p.grad_table) bucket_add<GEN, WEIGHTS>(bv, kv, sums, dp, s, kb, k0, qpos, half, far);
       column_product<T, DP>(kt, 32 * kb, dp, dq, lane);
     }
   }
   if (qi < p.nq)
     store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, dq, p.scale, p.dim, a.whole4, half);
+  // what dS add up to is delta's error (WEIGHTS): the second launch gets delta without it
+  const float all = WEIGHTS ? half_sum(sums.all) : 0.0f;
+  if (qi < p.nq && half == 0) a.delta[stat] = delta + all;
   if (p.grad_table) {
     if (!GEN) {
-      add_to<WEIGHTS>(sums, bv.map[0], sums.far_ds[0], sums.far_weight[0]);
-      add_to<WEIGHTS>(sums, bv.map[2 * p.radius + 128], sums.far_ds[1], sums.far_weight[1]);
+      const int t[2] = {bv.map[0], bv.map[2 * p.radius + 128]};
+      add_pair(sums.ds, t[0], sums.far_ds[0], t[1], sums.far_ds[1]);
+      for (int i = 0; WEIGHTS && i < 2; ++i) atomicAdd(sums.weight + 32 * t[i], fixed_weight(sums.far_weight[i]));
     }
-    const float all = half_sum(sums.all);
     if (half == 0) row_sum[32 * wave + lane] = all;
     __syncthreads();
     float* out = a.part + ((at.h * p.batch + at.b) * a.tiles + at.tile) * p.buckets;
     for (int t = threadIdx.x; t < p.buckets; t += ATT_NT) {
       float x = 0.0f, y = 0.0f;
       for (int w = 0; w < ATT_WAVES; ++w) {
+#pragma unroll 4
         for (int l = 0; l < 64; ++l) x += ds_sums[(w * p.buckets + t) * 64 + ((l + t) & 63)];  // rotated: no shared bank
         if (WEIGHTS)
+#pragma unroll 4
           for (int l = 0; l < 32; ++l) {
             const int r = (l + t) & 31;
             y += row_sum[32 * w + r] * (float)weights[(w * p.buckets + t) * 32 + r];
@@ -236,8 +246,7 @@ __device__ __forceinline__ v16f bias_block_t(const BiasView& bv, const QueryView
       const int q[4] = {qp.x, qp.y, qp.z, qp.w};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = __builtin_elementwise_sub_sat(kpos, q[r]);
-        x[4 * g + r] = bv.lut[bv.map[max(-bv.radius, min(bv.radius, d)) + bv.radius]];
+        x[4 * g + r] = bv.lut[distance_bucket(bv.map, bv.radius, kpos, q[r])];
       }
     }
   } else {
@@ -250,7 +259,7 @@ __device__ __forceinline__ v16f bias_block_t(const BiasView& bv, const QueryView
 }
 
 template <class T, int DP, bool GEN>
-__global__ __launch_bounds__(ATT_NT, 1) void attention_dkv_kernel(const AttArgs a) {
+__global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void attention_dkv_kernel(const AttArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention& p = a.p;
   constexpr int DB = DP / 32, TS = ATT_TILE * tile_stride<T>(DP);

@@ -7,8 +7,8 @@
 //
 // Gradient: d table[t, h] = sum of g over the pairs in bucket t. Bound by the reads. Each lane adds
 // to sums of its own in LDS, [bucket][lane], so that no two lanes meet in a bank and no order of
-// atomics enters the result: a wave's LDS operations complete in the order of issue. The lanes' and
-// then the workgroups' sums are added in a fixed order, the last in double.
+// atomics enters the result. The lanes' and then the workgroups' sums are added in a fixed order, the last in
+// double.
 #include "net.h"
 
 namespace fx {
@@ -27,37 +27,44 @@ struct BiasArgs {
   void* out;  // gradient: the workgroups' sums
 };
 
-// The vectors (sample b, row i, first key V chunk) that a thread takes, in steps of the whole
-// grid: the divisions are made once, a step only adds with carries.
-struct Walk {
-  int64_t b;
-  int i, chunk;  // chunk = first key / V
-  int64_t db;
-  int di, dchunk;
-  int nq, chunks;
-
-  __device__ __forceinline__ Walk(int64_t first, int64_t step, int nq_, int chunks_) : nq(nq_), chunks(chunks_) {
-    const int64_t row = first / chunks, drow = step / chunks;
-    chunk = (int)(first - row * chunks);
-    dchunk = (int)(step - drow * chunks);
-    b = row / nq;
-    i = (int)(row - b * nq);
-    db = drow / nq;
-    di = (int)(drow - db * nq);
-  }
-  __device__ __forceinline__ void next() {
-    chunk += dchunk;
-    const int c = chunk >= chunks;
-    chunk -= c ? chunks : 0;
-    i += di + c;
-    const int d = i >= nq;
-    i -= d ? nq : 0;
-    b += db + d;
+// How a workgroup of nt lanes goes over the pairs: 2^shift lanes take a row's vectors (of V keys) in turn, the rest
+// of it further rows; an item is BIAS_UNROLL x BIAS_TURNS such sets of rows of one sample. A lane's keys
+// then stay in registers for all rows of an item, and its rows' loads are in flight together.
+constexpr int BIAS_UNROLL = 4, BIAS_TURNS = 4;
+struct Tiling {
+  int shift, rows, item_rows;
+  int64_t items;  // of all samples
+  __host__ __device__ Tiling(int nt, int64_t batch, int nq, int chunks) {
+    shift = 0;
+    while ((1 << shift) < chunks && (2 << shift) <= nt) ++shift;
+    rows = nt >> shift;
+    item_rows = rows * BIAS_UNROLL * BIAS_TURNS;
+    items = batch * ((nq + item_rows - 1) / item_rows);
   }
 };
 
-__device__ __forceinline__ void stage_map(const BiasArgs& a, unsigned char* map) {
-  for (int i = threadIdx.x; i <= 2 * a.radius; i += BIAS_NT) map[i] = a.map[i];
+// The map, its entries within the table, into LDS.
+__device__ __forceinline__ void stage_map(const BiasArgs& a, unsigned char* map, int nt) {
+  for (int i = threadIdx.x; i <= 2 * a.radius; i += nt) map[i] = (unsigned char)min((int)a.map[i], a.buckets - 1);
+}
+
+// f(first row, end, first key) for each vector column of each of the workgroup's items; sample b.
+template <int V, class F>
+__device__ __forceinline__ void for_items(const BiasArgs& a, int nt, F&& f) {
+  const int chunks = a.nk / V;
+  const Tiling t(nt, a.batch, a.nq, chunks);
+  const int per = (a.nq + t.item_rows - 1) / t.item_rows, lane = threadIdx.x & ((1 << t.shift) - 1);
+  for (int64_t item = blockIdx.x; item < t.items; item += gridDim.x) {
+    const int64_t b = item / per;
+    const int r0 = (int)(item - b * per) * t.item_rows, r1 = min(a.nq, r0 + t.item_rows);
+    for (int c = lane; c < chunks; c += 1 << t.shift) f(b, r0 + (int)(threadIdx.x >> t.shift), r1, t.rows, c * V);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void load_keys(const int* p, int (&k)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) k[v] = p[v];
 }
 
 // V: elements of a store; 1 where rows of nk elements are not 16-byte aligned.
@@ -69,24 +76,28 @@ __global__ __launch_bounds__(BIAS_NT) void bias_kernel(const BiasArgs a) {
   const T* table = static_cast<const T*>(a.table);
   for (int i = threadIdx.x; i < a.heads * a.buckets; i += BIAS_NT)
     tab[i] = table[(i % a.buckets) * a.heads + i / a.buckets];
-  stage_map(a, map);
+  stage_map(a, map, BIAS_NT);
   __syncthreads();
-  T* out = static_cast<T*>(a.out);
-  for (Walk w((int64_t)blockIdx.x * BIAS_NT + threadIdx.x, (int64_t)gridDim.x * BIAS_NT, a.nq, a.nk / V); w.b < a.batch;
-       w.next()) {
-    const int q = a.q_pos[w.b * a.nq + w.i];
-    const int* kp = a.k_pos + w.b * a.nk + w.chunk * V;
-    int bucket[V];
+  for_items<V>(a, BIAS_NT, [&](int64_t b, int first, int end, int step, int key) {
+    int k[V];
+    load_keys<V>(a.k_pos + b * a.nk + key, k);
+    const int* qp = a.q_pos + b * a.nq;
+    T* const out = static_cast<T*>(a.out) + b * a.heads * a.nq * (int64_t)a.nk + key;
+#pragma unroll 2
+    for (int i = first; i < end; i += step) {
+      const int q = qp[i];
+      int bucket[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) bucket[v] = distance_bucket(map, a.radius, a.buckets, kp[v], q);
-    T* o = out + ((w.b * a.heads) * a.nq + w.i) * (int64_t)a.nk + w.chunk * V;
-    for (int h = 0; h < a.heads; ++h, o += (int64_t)a.nq * a.nk) {
-      vec_t<T, V> x;
+      for (int v = 0; v < V; ++v) bucket[v] = distance_bucket(map, a.radius, k[v], q);
+      T* o = out + (int64_t)i * a.nk;
+      for (int h = 0; h < a.heads; ++h, o += (int64_t)a.nq * a.nk) {
+        vec_t<T, V> x;
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = tab[h * a.buckets + bucket[v]];
-      *reinterpret_cast<vec_t<T, V>*>(o) = x;
+        for (int v = 0; v < V; ++v) x[v] = tab[h * a.buckets + bucket[v]];
+        *reinterpret_cast<vec_t<T, V>*>(o) = x;
+      }
     }
-  }
+  });
 }
 
 template <class T>
@@ -106,26 +117,39 @@ __global__ __launch_bounds__(64 * W) void bias_grad_kernel(const BiasArgs a) {
   A* sums = reinterpret_cast<A*>(smem);  // [wave][bucket][lane]
   unsigned char* map = smem + (size_t)W * a.buckets * 64 * sizeof(A);
   for (int i = threadIdx.x; i < W * a.buckets * 64; i += 64 * W) sums[i] = A(0);
-  for (int i = threadIdx.x; i <= 2 * a.radius; i += 64 * W) map[i] = a.map[i];
+  stage_map(a, map, 64 * W);
   __syncthreads();
   A* mine = sums + (threadIdx.x >> 6) * a.buckets * 64 + (threadIdx.x & 63);
   const int h = blockIdx.y;
-  const T* g = static_cast<const T*>(a.table);
-  for (Walk w((int64_t)blockIdx.x * 64 * W + threadIdx.x, (int64_t)gridDim.x * 64 * W, a.nq, a.nk / V); w.b < a.batch;
-       w.next()) {
-    const int q = a.q_pos[w.b * a.nq + w.i];
-    const int* kp = a.k_pos + w.b * a.nk + w.chunk * V;
-    const vec_t<T, V> x =
-        *reinterpret_cast<const vec_t<T, V>*>(g + ((w.b * a.heads + h) * a.nq + w.i) * (int64_t)a.nk + w.chunk * V);
+  for_items<V>(a, 64 * W, [&](int64_t b, int first, int end, int step, int key) {
+    int k[V];
+    load_keys<V>(a.k_pos + b * a.nk + key, k);
+    const int* qp = a.q_pos + b * a.nq;
+    const T* g = static_cast<const T*>(a.table) + (b * a.heads + h) * a.nq * (int64_t)a.nk + key;
+    for (int i = first; i < end; i += BIAS_UNROLL * step) {
+      vec_t<T, V> x[BIAS_UNROLL];
+      int q[BIAS_UNROLL];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      unsafeAtomicAdd(mine + distance_bucket(map, a.radius, a.buckets, kp[v], q) * 64, (A)x[v]);
-  }
+      for (int u = 0; u < BIAS_UNROLL; ++u) {
+        const int r = i + u * step;
+        x[u] = {};  // a row past the end adds zeros
+        q[u] = qp[min(r, end - 1)];
+        if (r < end) x[u] = *reinterpret_cast<const vec_t<T, V>*>(g + (int64_t)r * a.nk);
+      }
+      int t[BIAS_UNROLL * V];
+#pragma unroll
+      for (int j = 0; j < BIAS_UNROLL * V; ++j) t[j] = distance_bucket(map, a.radius, k[j % V], q[j / V]);
+#pragma unroll
+      for (int j = 0; j < BIAS_UNROLL * V; j += 2)
+        add_pair(mine, t[j], (A)x[j / V][j % V], t[j + 1], (A)x[(j + 1) / V][(j + 1) % V]);
+    }
+  });
   __syncthreads();
   A* out = static_cast<A*>(a.out) + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.buckets;
   for (int t = threadIdx.x; t < a.buckets; t += 64 * W) {
     A s = A(0);
     for (int w = 0; w < W; ++w)
+#pragma unroll 4
       for (int l = 0; l < 64; ++l) s += sums[(w * a.buckets + t) * 64 + ((l + t) & 63)];  // rotated: no shared bank
     out[t] = s;
   }
@@ -150,12 +174,10 @@ __global__ __launch_bounds__(BIAS_NT) void bucket_join_kernel(const A* part, int
 
 int bias_waves(int buckets) { return buckets <= 32 ? 4 : buckets <= 64 ? 2 : 1; }
 
-// Workgroups of a head in the gradient: as many as fit the card twice over, none with less than
-// one vector a lane.
-int64_t bias_grad_groups(int buckets, int64_t rows, int heads, int nk, int v) {
-  const int64_t nt = 64 * bias_waves(buckets);
-  const int64_t most = cdiv(rows * cdiv(nk, v), nt);
-  const int64_t fit = cdiv(2048, heads);
+// Workgroups of a head in the gradient: about what the card holds at once.
+int64_t bias_grad_groups(int buckets, int64_t batch, int heads, int nq, int nk, int v) {
+  const int64_t most = Tiling(64 * bias_waves(buckets), batch, nq, nk / v).items;
+  const int64_t fit = cdiv(1280, heads);
   return most < fit ? most : fit;
 }
 
@@ -201,7 +223,7 @@ int fx_relative_bias(const void* table, const uint8_t* map, int32_t radius, int3
     using T = decltype(t);
     constexpr int V = VEC16<T>;
     const int v = bias_vec(nk, sizeof(T), out);
-    const int64_t most = cdiv(batch * nq * cdiv(nk, v), BIAS_NT);
+    const int64_t most = Tiling(BIAS_NT, batch, nq, nk / v).items;
     const unsigned grid = (unsigned)(most < 4096 ? most : 4096);
     const size_t lds = (size_t)heads * buckets * sizeof(T) + 2 * radius + 1;
     if (v == V)
@@ -216,7 +238,7 @@ size_t fx_relative_bias_grad_workspace(int32_t buckets, int64_t batch, int32_t h
                                        int32_t dtype) {
   if (!bias_sizes_ok(0, buckets, batch, heads, nq, nk, dtype) || batch == 0 || nq == 0 || nk == 0) return 0;
   // of the scalar kernel, which has the most workgroups
-  return (size_t)bias_grad_groups(buckets, batch * nq, heads, nk, 1) * heads * buckets * (dtype == FX_F64 ? 8 : 4);
+  return (size_t)bias_grad_groups(buckets, batch, heads, nq, nk, 1) * heads * buckets * (dtype == FX_F64 ? 8 : 4);
 }
 
 int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radius, int32_t buckets,
@@ -243,7 +265,7 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
       const int v = bias_vec(nk, sizeof(T), grad_out);
       const BiasArgs a{grad_out, map, radius, buckets, q_pos, k_pos, batch, heads, nq, nk, workspace};
       const int w = bias_waves(buckets);
-      groups = bias_grad_groups(buckets, batch * nq, heads, nk, v);
+      groups = bias_grad_groups(buckets, batch, heads, nq, nk, v);
       const size_t lds = (size_t)w * buckets * 64 * sizeof(A) + 2 * radius + 1;
       const dim3 grid((unsigned)groups, heads);
       auto go = [&](auto vv, auto ww) {

@@ -30,12 +30,25 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// Distance buckets: map[clamp(d, -radius, radius) + radius], clamped to the table's last row. The
-// distance saturates, so positions of any int32 value are in order.
-__device__ __forceinline__ int distance_bucket(const unsigned char* map, int radius, int buckets, int kpos, int qpos) {
+// Distance buckets: map[clamp(d, -radius, radius) + radius] (map staged with its entries within the table).
+// The distance saturates, so positions of any int32 value are in order.
+__device__ __forceinline__ int distance_bucket(const unsigned char* map, int radius, int kpos, int qpos) {
   const int d = __builtin_elementwise_sub_sat(kpos, qpos);
-  const int at = max(-radius, min(radius, d)) + radius;
-  return min((int)map[at], buckets - 1);
+  return map[max(-radius, min(radius, d)) + radius];
+}
+
+// Adds to two of a lane's own sums in LDS, [bucket][64 lanes]: no two lanes share a word or a bank, and the
+// order is that of the program. Reading, adding and writing takes 8 clk of a CU for a wave, ds_add_f32 193. The
+// second read does not wait for the first write; where both are one word the sum is carried over.
+template <class A>
+__device__ __forceinline__ void add_pair(A* mine, int t0, A x0, int t1, A x1) {
+  A* const p0 = mine + 64 * t0;
+  A* const p1 = mine + 64 * t1;
+  const A a = *p0, b = *p1;
+  x0 += a;
+  x1 += t1 == t0 ? x0 : b;
+  *p0 = x0;
+  *p1 = x1;
 }
 
 inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
