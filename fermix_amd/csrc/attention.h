@@ -197,14 +197,8 @@ __device__ __forceinline__ void column_product(const T* tile, int row0, const v1
 }
 
 // Maximum and sum of the lane's value and that of the lane 32 away.
-__device__ __forceinline__ float half_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
+__device__ __forceinline__ float half_max(float x) { return join32<MaxOp>(x); }
+__device__ __forceinline__ float half_sum(float x) { return join32<AddOp>(x); }
 
 // A transposed accumulator (rows: 32 d + .. columns of the result; column: the lane's row) times f, as
 // rows of memory.

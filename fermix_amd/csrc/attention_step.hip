@@ -1,12 +1,14 @@
 // Attention of one new token a sample over a paged key-value cache, with the relative position bias.
 //
-// Bound by reading the cache once. A workgroup takes one kv head of a sample and a part of its
-// tokens; the LPT lanes that hold a 16-byte vector each make up a token's row, a wave reads 64 / LPT
-// tokens at a time, four times over, straight into registers (K and V are used once, LDS would
-// only delay them). The lanes of a row add up its scores for all the heads that share it; each row
-// position of the wave keeps a running maximum and sum of its own, joined at the end. Where there are
-// few samples the tokens are split over workgroups (as evenly as the sample's own length allows), whose
-// sums a second launch joins.
+// Bound by reading the cache once. The LPT lanes that hold a 16-byte vector each make up a token's row, a wave
+// reads 64 / LPT tokens at a time, four times over, straight into registers (K and V are used once, LDS
+// would only delay them), with the next tokens' rows and the page numbers after those already on their way.
+// The lanes of a row add up its scores for all the heads that share it; each row position of the wave keeps a
+// running maximum and sum of its own, joined at the end by lane moves.
+//
+// With many samples a wave takes a kv head of a sample by itself. With few, four waves take it together, and
+// where that is not enough either its tokens are split over workgroups (as evenly as the sample's own length
+// allows), whose sums a second launch joins. The order of all sums depends on sizes and lengths alone.
 #include "net.h"
 
 namespace fx {
@@ -33,20 +35,44 @@ __device__ __forceinline__ float log2_bias(float b) {
   return isinf(b) || !(fabsf(x) > F32_MAX) ? x : copysignf(F32_MAX, b);
 }
 
-template <class T, int DP, int G>
-__global__ __launch_bounds__(STEP_NT) void step_kernel(const StepArgs a) {
-  constexpr int V = VEC16<T>, LPT = DP / V, ROWS = 64 / LPT, U = 4;
+template <int V, class T>
+__device__ __forceinline__ void widen(const vec_t<T, V>& x, float (&y)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) y[e] = (float)x[e];
+}
+
+// A token's vector of this lane; elements past dim are zero.
+template <class T>
+__device__ __forceinline__ vec_t<T, VEC16<T>> load_part(const T* row, int d0, int dim, bool vec) {
+  constexpr int V = VEC16<T>;
+  vec_t<T, V> x = {};
+  if (vec) {
+    if (d0 < dim) x = *reinterpret_cast<const vec_t<T, V>*>(row + d0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (d0 + e < dim) x[e] = row[d0 + e];
+  }
+  return x;
+}
+
+// G: heads at a time. W: waves that share a unit (a block of G heads of a kv head of a sample), 1 or 4.
+template <class T, int DP, int G, int W>
+__global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
+  constexpr int V = VEC16<T>, LPT = DP / V, ROWS = 64 / LPT, U = 4, STRIDE = W * ROWS * U;
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention_step& p = a.p;
-  float* const acc_lds = reinterpret_cast<float*>(smem);           // [wave][G][DP]
-  float2* const stat_lds = reinterpret_cast<float2*>(acc_lds + STEP_WAVES * G * DP);  // [wave][G]
-  float* const tab = reinterpret_cast<float*>(stat_lds + STEP_WAVES * G);             // [G][buckets]
-  unsigned char* const map = reinterpret_cast<unsigned char*>(tab + G * p.buckets);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = W == 1 ? wave : 0;
+  float* const acc_lds = reinterpret_cast<float*>(smem);                                 // [wave][G][DP] (W > 1)
+  float2* const stat_lds = reinterpret_cast<float2*>(acc_lds + (W > 1 ? W * G * DP : 0));  // [wave][G] (W > 1)
+  float* const tabs = reinterpret_cast<float*>(stat_lds + (W > 1 ? W * G : 0));            // [unit][G][buckets]
+  unsigned char* const map = reinterpret_cast<unsigned char*>(tabs + (W == 1 ? STEP_WAVES : 1) * G * p.buckets);
+  float* const tab = tabs + mine * G * p.buckets;
 
-  const int group = p.heads / p.kv_heads, blocks = (group + G - 1) / G;
-  const int split = blockIdx.x;
-  const int kh = blockIdx.y / blocks, h0 = kh * group + (blockIdx.y % blocks) * G;
-  const int heads = min(G, group - (int)(blockIdx.y % blocks) * G);
+  const int group = p.heads / p.kv_heads, blocks = (group + G - 1) / G, units = p.kv_heads * blocks;
+  const int split = blockIdx.x, unit = min(units - 1, W == 1 ? (int)blockIdx.y * STEP_WAVES + wave : (int)blockIdx.y);
+  const bool spare = W == 1 && (int)blockIdx.y * STEP_WAVES + wave >= units;  // a wave without a unit
+  const int kh = unit / blocks, h0 = kh * group + (unit % blocks) * G, heads = min(G, group - (unit % blocks) * G);
   const int64_t b = blockIdx.z;
   const int len = p.lengths[b];
   const int n = p.k ? (len < 0 ? 0 : len == 0x7fffffff ? len : len + 1) : max(len, 0);  // tokens attended to
@@ -55,13 +81,59 @@ __global__ __launch_bounds__(STEP_NT) void step_kernel(const StepArgs a) {
   per = (int)min((int64_t)n, ((int64_t)per + a.unit - 1) / a.unit * a.unit);
   const int64_t t0 = (int64_t)split * per, t1 = over ? 0 : min((int64_t)n, t0 + per);
   const int64_t row0 = (b * p.heads + h0) * a.splits + split;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = lane % LPT, d0 = part * V;
+  const int part = lane % LPT, d0 = part * V, row = lane / LPT;
   if (t0 >= t1 && a.splits > 1 && !over) {
     if ((int)threadIdx.x < heads) a.stat[row0 + (int64_t)threadIdx.x * a.splits] = make_float2(-INFINITY, 0.0f);
     return;
   }
+
+  const bool own = p.k && t1 == n && n > 0;  // this part has the new token, which is in the call, not the cache
+  const int64_t end = own ? t1 - 1 : t1;     // of the cached tokens
+  const int64_t row_size = (int64_t)p.kv_heads * p.dim;
+  const T* const kc = static_cast<const T*>(p.k_cache) + (int64_t)kh * p.dim;
+  const T* const vc = static_cast<const T*>(p.v_cache) + (int64_t)kh * p.dim;
+  const int* const table = p.page_table + b * p.max_pages;
+  bool bad = over;
+  // where a token's row is, in elements; -1 for a page outside the cache
+  auto slot_of = [&](int64_t t) -> int64_t {
+    const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)t * a.magic) >> a.shift);
+    const int page = table[pg];
+    if ((uint32_t)page >= (uint64_t)p.pages) return -1;
+    return ((int64_t)page * p.page_size + ((uint32_t)t - pg * (uint32_t)p.page_size)) * row_size;
+  };
+  const int64_t first = t0 + (W == 1 ? 0 : wave * ROWS * U);
+  int64_t slot[U];
+  vec_t<T, V> k[U], v[U], nk[U], nv[U];
+  auto find = [&](int64_t base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = base + u * ROWS + row;
+      slot[u] = -1;
+      if (t < end) {
+        slot[u] = slot_of(t);
+        if (slot[u] < 0) bad = true;
+      }
+    }
+  };
+  auto fetch = [&](vec_t<T, V>(&x)[U], vec_t<T, V>(&y)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = y[u] = {};
+      if (slot[u] >= 0) {
+        x[u] = load_part<T>(kc + slot[u], d0, p.dim, a.vec);
+        y[u] = load_part<T>(vc + slot[u], d0, p.dim, a.vec);
+      }
+    }
+  };
+  find(first);
+  if (W > 1) {
+    fetch(k, v);
+    find(first + STRIDE);
+  }
+
   if (p.table) {
-    for (int i = threadIdx.x; i < heads * p.buckets; i += STEP_NT)
+    const int at = W == 1 ? lane : threadIdx.x, nt = W == 1 ? 64 : STEP_NT;
+    for (int i = at; i < heads * p.buckets; i += nt)
       tab[i] = log2_bias(p.table[(int64_t)(i % p.buckets) * p.heads + h0 + i / p.buckets]);
     for (int i = threadIdx.x; i <= p.radius; i += STEP_NT) map[i] = (unsigned char)min((int)p.map[i], p.buckets - 1);
   }
@@ -71,83 +143,94 @@ __global__ __launch_bounds__(STEP_NT) void step_kernel(const StepArgs a) {
   for (int g = 0; g < G; ++g) {
     m[g] = -INFINITY;
     l[g] = 0.0f;
+    vec_t<T, V> x = {};
+    if (g < heads) x = load_part<T>(static_cast<const T*>(p.q) + (b * p.heads + h0 + g) * p.dim, d0, p.dim, false);
+    widen<V>(x, q[g]);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       acc[g][e] = 0.0f;
-      q[g][e] = g < heads && d0 + e < p.dim ? c * (float)static_cast<const T*>(p.q)[(b * p.heads + h0 + g) * p.dim + d0 + e] : 0.0f;
+      q[g][e] *= c;
     }
   }
-  bool bad = over;
   __syncthreads();
 
-  const int64_t row_size = (int64_t)p.kv_heads * p.dim;
-  const T* const kc = static_cast<const T*>(p.k_cache) + (int64_t)kh * p.dim;
-  const T* const vc = static_cast<const T*>(p.v_cache) + (int64_t)kh * p.dim;
-  const int* const table = p.page_table + b * p.max_pages;
-  auto load = [&](const T* src, float (&x)[V]) {
-    if (a.vec) {
-      vec_t<T, V> v = {};
-      if (d0 < p.dim) v = *reinterpret_cast<const vec_t<T, V>*>(src + d0);
+  if (own && !spare) {
+    // the new token: into the cache (by the first wave of the kv head's first heads), and the start of the sums
+    // of the wave's first row position
+    const int64_t at = (b * p.kv_heads + kh) * p.dim;
+    const vec_t<T, V> xk = load_part<T>(static_cast<const T*>(p.k) + at, d0, p.dim, false);
+    const vec_t<T, V> xv = load_part<T>(static_cast<const T*>(p.v) + at, d0, p.dim, false);
+    const int64_t to = slot_of(n - 1);
+    if (to < 0) bad = true;
+    if (W == 1 || wave == 0) {
+      if (to >= 0 && unit % blocks == 0 && row == 0) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[e] = (float)v[e];
-    } else {
+        for (int e = 0; e < V; ++e)
+          if (d0 + e < p.dim) {
+            static_cast<T*>(p.k_cache)[to + (int64_t)kh * p.dim + d0 + e] = xk[e];
+            static_cast<T*>(p.v_cache)[to + (int64_t)kh * p.dim + d0 + e] = xv[e];
+          }
+      }
+      float kf[V], vf[V];
+      widen<V>(xk, kf);
+      widen<V>(xv, vf);
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[e] = d0 + e < p.dim ? (float)src[d0 + e] : 0.0f;
+      for (int g = 0; g < G; ++g) {
+        if (g >= heads) break;
+        float x = 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) x += q[g][e] * kf[e];
+        x = group_sum<LPT>(x);
+        if (p.table) x += tab[g * p.buckets + map[p.radius]];
+        if (row == 0 && x != -INFINITY) {
+          m[g] = x;
+          l[g] = 1.0f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[g][e] = vf[e];
+        }
+      }
     }
-  };
-  for (int64_t base = t0 + wave * ROWS; base < t1; base += STEP_WAVES * ROWS * U) {
-    float k[U][V], v[U][V];
-    bool on[U];
+  }
+
+  for (int64_t base = first; base < end; base += STRIDE) {
+    if (W > 1) {
+      fetch(nk, nv);
+      find(base + 2 * STRIDE);
+    } else {
+      fetch(k, v);
+      find(base + STRIDE);
+    }
+    float s[U][G];
     int dist[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t t = base + u * STEP_WAVES * ROWS + lane / LPT;
-      on[u] = t < t1;
-      dist[u] = (int)(t - (n - 1));
+      float kf[V];
+      widen<V>(k[u], kf);
+      dist[u] = max((int)(base + u * ROWS + row - (n - 1)), -p.radius) + p.radius;
 #pragma unroll
-      for (int e = 0; e < V; ++e) k[u][e] = v[u][e] = 0.0f;
-      if (!on[u]) continue;
-      const T *ks, *vs;
-      const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)t * a.magic) >> a.shift);
-      const int page = table[pg];
-      const bool ok = (uint32_t)page < (uint64_t)p.pages;
-      if (!ok) {
-        bad = true;
-        continue;
-      }
-      const int64_t slot = ((int64_t)page * p.page_size + ((uint32_t)t - pg * (uint32_t)p.page_size)) * row_size;
-      if (p.k && t == n - 1) {
-        // the new token: from the call, and into the cache once (by the group's first heads)
-        ks = static_cast<const T*>(p.k) + (b * p.kv_heads + kh) * p.dim;
-        vs = static_cast<const T*>(p.v) + (b * p.kv_heads + kh) * p.dim;
-        if (blockIdx.y % blocks == 0) {
+      for (int g = 0; g < G; ++g) {
+        float x = 0.0f;
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (d0 + e < p.dim) {
-              static_cast<T*>(p.k_cache)[slot + (int64_t)kh * p.dim + d0 + e] = ks[d0 + e];
-              static_cast<T*>(p.v_cache)[slot + (int64_t)kh * p.dim + d0 + e] = vs[d0 + e];
-            }
-        }
-      } else {
-        ks = kc + slot;
-        vs = vc + slot;
+        for (int e = 0; e < V; ++e) x += q[g][e] * kf[e];
+        s[u][g] = group_sum<LPT>(x);
       }
-      load(ks, k[u]);
-      load(vs, v[u]);
+    }
+    if (p.table) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = map[min(dist[u], p.radius)];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (g < heads) s[u][g] += tab[g * p.buckets + t];
+      }
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      if (g >= heads) break;
-      float s[U], top = m[g];
+      float top = m[g];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float x = 0.0f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) x += q[g][e] * k[u][e];
-        x = group_sum<LPT>(x);
-        if (p.table && on[u]) x += tab[g * p.buckets + map[max(dist[u], -p.radius) + p.radius]];
-        s[u] = on[u] ? x : -INFINITY;
-        top = fmaxf(top, s[u]);
+        if (base + u * ROWS + row >= end) s[u][g] = -INFINITY;
+        top = fmaxf(top, s[u][g]);
       }
       const float at = top == -INFINITY ? 0.0f : top;
       const float keep = __builtin_amdgcn_exp2f(m[g] - at);
@@ -157,78 +240,130 @@ __global__ __launch_bounds__(STEP_NT) void step_kernel(const StepArgs a) {
       for (int e = 0; e < V; ++e) acc[g][e] *= keep;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float w = __builtin_amdgcn_exp2f(s[u] - at);
-        l[g] += w;
+        s[u][g] = __builtin_amdgcn_exp2f(s[u][g] - at);
+        l[g] += s[u][g];
+      }
+    }
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[g][e] += w * v[u][e];
+    for (int u = 0; u < U; ++u) {
+      float vf[V];
+      widen<V>(v[u], vf);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[g][e] += s[u][g] * vf[e];
+      if (W > 1) {
+        k[u] = nk[u];
+        v[u] = nv[u];
       }
     }
   }
 
-  // the wave's row positions, then the waves
+  // the wave's row positions
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    float top = m[g];
+    const float top = stride_join<LPT, MaxOp>(m[g]);
+    const float keep = __builtin_amdgcn_exp2f(m[g] - (top == -INFINITY ? 0.0f : top));
+    m[g] = top;
+    l[g] = stride_join<LPT, AddOp>(l[g] * keep);
 #pragma unroll
-    for (int x = LPT; x < 64; x <<= 1) top = fmaxf(top, shfl_xor(top, x));
-    const float at = top == -INFINITY ? 0.0f : top;
-    const float keep = __builtin_amdgcn_exp2f(m[g] - at);
-    l[g] *= keep;
-#pragma unroll
-    for (int x = LPT; x < 64; x <<= 1) l[g] += shfl_xor(l[g], x);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      acc[g][e] *= keep;
-#pragma unroll
-      for (int x = LPT; x < 64; x <<= 1) acc[g][e] += shfl_xor(acc[g][e], x);
-      if (lane < LPT) acc_lds[(wave * G + g) * DP + d0 + e] = acc[g][e];
-    }
-    if (lane == 0) stat_lds[wave * G + g] = make_float2(top, l[g]);
+    for (int e = 0; e < V; ++e) acc[g][e] = stride_join<LPT, AddOp>(acc[g][e] * keep);
   }
-  const bool any_bad = __syncthreads_or(bad);
-  for (int i = threadIdx.x; i < heads * DP; i += STEP_NT) {
-    const int g = i / DP, d = i % DP;
-    float top = -INFINITY, sum = 0.0f, x = 0.0f;
-    for (int w = 0; w < STEP_WAVES; ++w) top = fmaxf(top, stat_lds[w * G + g].x);
-    for (int w = 0; w < STEP_WAVES; ++w) {
-      const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat_lds[w * G + g].x - top);
-      sum += f * stat_lds[w * G + g].y;
-      x += f * acc_lds[(w * G + g) * DP + d];
+  if constexpr (W == 1) {
+    bad = __any(bad);
+    if (spare || row != 0) return;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (g >= heads) break;
+      const float inv = bad ? NAN : l[g] == 0.0f ? 0.0f : 1.0f / l[g];
+      T* o = static_cast<T*>(p.out) + (b * p.heads + h0 + g) * p.dim + d0;
+      vec_t<T, V> x;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = (T)(acc[g][e] * inv);
+      if (a.vec) {
+        if (d0 < p.dim) *reinterpret_cast<vec_t<T, V>*>(o) = x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (d0 + e < p.dim) o[e] = x[e];
+      }
     }
-    if (any_bad) x = sum = NAN;
-    if (d >= p.dim) continue;
-    if (a.splits == 1) {
-      static_cast<T*>(p.out)[(b * p.heads + h0 + g) * p.dim + d] = (T)(sum == 0.0f ? 0.0f : x / sum);
-    } else {
-      const int64_t r = row0 + (int64_t)g * a.splits;
-      a.part[r * p.dim + d] = x;
-      if (d == 0) a.stat[r] = make_float2(any_bad ? NAN : top, sum);
+    return;
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (row == 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc_lds[(wave * G + g) * DP + d0 + e] = acc[g][e];
+      }
+      if (lane == 0) stat_lds[wave * G + g] = make_float2(m[g], l[g]);
+    }
+    const bool any_bad = __syncthreads_or(bad);
+    for (int i = threadIdx.x; i < heads * DP; i += STEP_NT) {
+      const int g = i / DP, d = i % DP;
+      float top = -INFINITY, sum = 0.0f, x = 0.0f;
+      for (int w = 0; w < W; ++w) top = fmaxf(top, stat_lds[w * G + g].x);
+      for (int w = 0; w < W; ++w) {
+        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat_lds[w * G + g].x - top);
+        sum += f * stat_lds[w * G + g].y;
+        x += f * acc_lds[(w * G + g) * DP + d];
+      }
+      if (any_bad) x = sum = NAN;
+      if (d >= p.dim) continue;
+      if (a.splits == 1) {
+        static_cast<T*>(p.out)[(b * p.heads + h0 + g) * p.dim + d] = (T)(sum == 0.0f ? 0.0f : x / sum);
+      } else {
+        const int64_t r = row0 + (int64_t)g * a.splits;
+        a.part[r * p.dim + d] = x;
+        if (d == 0) a.stat[r] = make_float2(any_bad ? NAN : top, sum);
+      }
     }
   }
 }
 
-// One row of heads x dim a wave: the parts in order.
+// One (sample, head) a workgroup: the parts' weights by the first wave, then each lane a column of a share of the
+// parts, the shares joined in order.
 template <class T>
 __global__ __launch_bounds__(STEP_NT) void step_join_kernel(const StepArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * STEP_WAVES + (threadIdx.x >> 6);
-  if (row >= a.p.batch * a.p.heads) return;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* const weight = reinterpret_cast<float*>(smem);  // [splits]
+  float* const sums = weight + a.splits;                 // [share][dim]
+  __shared__ float inv;
+  const int64_t row = blockIdx.x;
   const float2* st = a.stat + row * a.splits;
-  float top = -INFINITY;
-  bool bad = false;
-  for (int i = 0; i < a.splits; ++i) {
-    bad |= st[i].x != st[i].x;
-    top = fmaxf(top, st[i].x);
-  }
-  for (int d = threadIdx.x & 63; d < a.p.dim; d += 64) {
-    float x = 0.0f, sum = 0.0f;
-    for (int i = 0; i < a.splits; ++i) {
-      if (st[i].y == 0.0f) continue;
-      const float f = __builtin_amdgcn_exp2f(st[i].x - top);
-      sum += f * st[i].y;
-      x += f * a.part[(row * a.splits + i) * a.p.dim + d];
+  if (threadIdx.x < 64) {
+    float top = -INFINITY, sum = 0.0f;
+    bool bad = false;
+    for (int i = threadIdx.x; i < a.splits; i += 64) {
+      bad |= st[i].x != st[i].x;
+      top = fmaxf(top, st[i].x);
     }
-    if (bad) x = sum = NAN;
-    static_cast<T*>(a.p.out)[row * a.p.dim + d] = (T)(sum == 0.0f ? 0.0f : x / sum);
+    top = join32<MaxOp>(join16<MaxOp>(stride_join<1, MaxOp>(top)));
+    for (int i = threadIdx.x; i < a.splits; i += 64) {
+      const float f = st[i].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(st[i].x - top);
+      weight[i] = f;
+      sum += f * st[i].y;
+    }
+    sum = group_sum<64>(sum);
+    bad = __any(bad);
+    if (threadIdx.x == 0) inv = bad ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+  }
+  __syncthreads();
+  const int dim = a.p.dim, shares = STEP_NT / dim, share = threadIdx.x / dim, d = threadIdx.x % dim;
+  if (share < shares) {
+    float x = 0.0f;
+#pragma unroll 4
+    for (int i = share; i < a.splits; i += shares) {
+      const float f = weight[i];
+      if (f != 0.0f) x += f * a.part[(row * a.splits + i) * dim + d];  // a part of weight 0 may hold nothing
+    }
+    sums[share * dim + d] = x;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < dim) {
+    float x = 0.0f;
+    for (int i = 0; i < shares; ++i) x += sums[i * dim + d];
+    static_cast<T*>(a.p.out)[row * dim + d] = (T)(x * inv);
   }
 }
 
@@ -243,6 +378,9 @@ bool step_sizes_ok(const fx_attention_step* p) {
 }
 
 int step_heads(int group) { return group >= 3 ? 4 : group; }  // heads that a workgroup takes at once
+
+// Units (samples x kv heads x blocks of their heads) from which each gets one wave: four waves a SIMD of the card.
+constexpr int64_t STEP_ALONE = 4096;
 
 // Parts of a sample's tokens: enough workgroups for the card, none under 256 tokens of the longest sample
 // that the table can hold.
@@ -291,6 +429,7 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
     return FX_ERR_WORKSPACE;
   const int group = p->heads / p->kv_heads, per = step_heads(group);
   const int64_t rows = p->kv_heads * cdiv(group, per);
+  const bool alone = p->batch * rows >= STEP_ALONE;
   if (rows > 65535 || (int64_t)p->max_pages * p->page_size > 0x7fffffff) return FX_ERR_UNSUPPORTED;
 
   StepArgs a{};
@@ -298,7 +437,7 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
   a.splits = splits;
   a.unit = 64;
   a.vec = p->dim % (16 / (int)e) == 0 && aligned(p->k_cache, 16) && aligned(p->v_cache, 16) && aligned(p->k, 16) &&
-          aligned(p->v, 16);
+          aligned(p->v, 16) && aligned(p->out, 16);
   int bits = 0;  // ceil(log2 page_size)
   while ((1ll << bits) < p->page_size) ++bits;
   a.shift = 31 + bits;
@@ -323,8 +462,13 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
       if (p->page_table) c.p.page_table = p->page_table + b0 * p->max_pages;
       auto go = [&](auto dp, auto g) {
         constexpr int DP = decltype(dp)::value, G = decltype(g)::value;
-        const size_t lds = 4 * STEP_WAVES * G * DP + 8 * STEP_WAVES * G + 4 * (size_t)G * p->buckets + p->radius + 1;
-        hipLaunchKernelGGL((step_kernel<T, DP, G>), dim3(splits, (unsigned)rows, (unsigned)nb), dim3(STEP_NT), lds, s, c);
+        const size_t tab = 4 * (size_t)G * p->buckets, map = p->radius + 1;
+        if (alone)
+          hipLaunchKernelGGL((step_kernel<T, DP, G, 1>), dim3(1, (unsigned)cdiv(rows, STEP_WAVES), (unsigned)nb),
+                             dim3(STEP_NT), STEP_WAVES * tab + map, s, c);
+        else
+          hipLaunchKernelGGL((step_kernel<T, DP, G, STEP_WAVES>), dim3(splits, (unsigned)rows, (unsigned)nb),
+                             dim3(STEP_NT), STEP_WAVES * G * (4 * DP + 8) + tab + map, s, c);
       };
       auto by_heads = [&](auto dp) {
         if (per == 1)
@@ -344,7 +488,8 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
         by_heads(ic<128>{});
       if (launched() != FX_OK) return FX_ERR_LAUNCH;
       if (splits > 1)
-        hipLaunchKernelGGL((step_join_kernel<T>), dim3((unsigned)cdiv(nb * p->heads, STEP_WAVES)), dim3(STEP_NT), 0, s, c);
+        hipLaunchKernelGGL((step_join_kernel<T>), dim3((unsigned)(nb * p->heads)), dim3(STEP_NT),
+                           sizeof(float) * (splits + STEP_NT), s, c);
     }
     return launched();
   });

@@ -20,13 +20,52 @@ __device__ __forceinline__ float to_f32(T x) {
 template <class T>
 constexpr int VEC16 = 16 / (int)sizeof(T);
 
-__device__ __forceinline__ float shfl_xor(float x, int m) { return __shfl_xor(x, m, 64); }
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+  return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(x)));
+}
 
-// Sum over the aligned group of W lanes (W a power of two up to 64); every lane gets it.
+struct AddOp {
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct MaxOp {
+  static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+};
+
+// x joined with that of the lane 16 or 32 away.
+template <class OP>
+__device__ __forceinline__ float join16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return OP::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <class OP>
+__device__ __forceinline__ float join32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return OP::of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Sum over the aligned group of W lanes (W a power of two up to 64); every lane gets it. No LDS: quad
+// permutes, mirrors, then swaps of rows.
 template <int W>
 __device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int m = W / 2; m; m >>= 1) x += shfl_xor(x, m);
+  if constexpr (W >= 2) x += dpp_f32<0xB1>(x);   // quad_perm [1,0,3,2]
+  if constexpr (W >= 4) x += dpp_f32<0x4E>(x);   // quad_perm [2,3,0,1]
+  if constexpr (W >= 8) x += dpp_f32<0x141>(x);  // row_half_mirror
+  if constexpr (W >= 16) x += dpp_f32<0x140>(x); // row_mirror
+  if constexpr (W >= 32) x = join16<AddOp>(x);
+  if constexpr (W >= 64) x = join32<AddOp>(x);
+  return x;
+}
+
+// x joined over the lanes that are equal modulo W (W a power of two): rotations within 16 lanes, then swaps.
+template <int W, class OP>
+__device__ __forceinline__ float stride_join(float x) {
+  if constexpr (W <= 8) x = OP::of(x, dpp_f32<0x128>(x));  // row_ror:8
+  if constexpr (W <= 4) x = OP::of(x, dpp_f32<0x124>(x));
+  if constexpr (W <= 2) x = OP::of(x, dpp_f32<0x122>(x));
+  if constexpr (W <= 1) x = OP::of(x, dpp_f32<0x121>(x));
+  if constexpr (W <= 16) x = join16<OP>(x);
+  if constexpr (W <= 32) x = join32<OP>(x);
   return x;
 }
 
