@@ -23,63 +23,6 @@ template <class T, int DP>
 constexpr size_t tiles_lds() {
   return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T);
 }
-constexpr size_t view_lds(bool gen, int radius, int buckets) {
-  return ((gen ? 4 * (size_t)buckets : 4 * (size_t)bias_entries(false, radius)) + bias_entries(gen, radius) + 15) / 16 * 16;
-}
-
-// The lane's bucket sums: of dS, of its query's P (WEIGHTS: the 16-bit types), and what tiles past the
-// radius add to the first and the last distance's bucket.
-struct Sums {
-  float* ds;
-  unsigned* weight;
-  float all;                    // of dS over all buckets
-  float far_ds[2], far_weight[2];  // below, above
-};
-__device__ __forceinline__ unsigned fixed_weight(float p) { return (unsigned)(p * 0x1p30f); }
-
-// Adds a block's dS and P (rows: keys; column: the lane's query).
-template <bool GEN, bool WEIGHTS>
-__device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv, Sums& sums, const v16f& ds,
-                                           const v16f& w, int kb, int k0, int qpos, int half, int far) {
-  if (!GEN && far) {
-    float total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) total += ds[i];
-    sums.far_ds[far > 0] += total;
-    if (WEIGHTS) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sums.far_weight[far > 0] += w[i];
-    }
-    return;
-  }
-  // all lookups before the first add: the compiler keeps a read that follows one behind it
-  int t[16];
-  if constexpr (GEN) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int4 kp = *reinterpret_cast<const int4*>(kv.pos + 32 * kb + 8 * g + 4 * half);
-      const int k[4] = {kp.x, kp.y, kp.z, kp.w};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        t[4 * g + r] = distance_bucket(bv.map, bv.radius, k[r], qpos);
-      }
-    }
-  } else {
-    const int d = max(-(bv.radius + 64), min(bv.radius, k0 - qpos));
-    const unsigned char* l = bv.map + d + bv.radius + 64 + 32 * kb + 4 * half;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = l[acc_row(i)];
-  }
-#pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    add_pair(sums.ds, t[i], ds[i], t[i + 1], ds[i + 1]);
-    if (WEIGHTS) {
-      atomicAdd(sums.weight + 32 * t[i], fixed_weight(w[i]));
-      atomicAdd(sums.weight + 32 * t[i + 1], fixed_weight(w[i + 1]));
-    }
-  }
-}
-
 template <class T, int DP, bool GEN>
 __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void attention_dq_kernel(const AttArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -406,6 +349,15 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
   }
   if (p->nk > 0 && (!p->k || !p->v || !p->grad_k || !p->grad_v)) return FX_ERR_INVALID_ARGUMENT;
   AttArgs a = attention_args(*p);
+  if (attention_grad_short_fits(*p)) {
+    a.part = static_cast<float*>(workspace);
+    a.tiles = 1;
+    a.items = p->batch * p->heads;
+    if (a.items > 0x7fffffff) return FX_ERR_UNSUPPORTED;
+    const int st = launch_attention_grad_short(a, s);
+    if (st != FX_OK || !p->grad_table) return st;
+    return launch_bucket_join(a.part, p->batch, p->buckets, p->heads, p->grad_table, s);
+  }
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + delta_floats(*p);
   const int qtiles = (int)cdiv(p->nq, 32 * ATT_WAVES), ktiles = (int)cdiv(p->nk, 32 * ATT_WAVES);

@@ -1,0 +1,230 @@
+// Attention's gradient in one launch, for sequences of up to 128 queries and keys of the 16-bit types.
+//
+// A workgroup has one head of a sample, a wave 32 of its queries, one to a lane as in the forward, with the
+// scores' and dP's transposed products of all keys in registers. So delta = sum P dP is exact where it is
+// needed: `out` is not read, dS add up to zero, the bucket sums need no correction. dq comes from the
+// wave's own dS; dk and dv contract over all queries: P, then dS, go through LDS, rounded, as [query][key],
+// beside the waves' query and cotangent rows, and a wave takes 32 of the keys. Five products, each tensor read
+// or written once: bound by memory.
+#include "attention.h"
+
+namespace fx {
+namespace net {
+namespace {
+
+constexpr int SHORT = 128;  // queries and keys
+
+template <class T, int DP>
+constexpr size_t short_tile() {
+  return (size_t)SHORT * tile_stride<T>(DP) * sizeof(T);
+}
+constexpr int PS = SHORT + 8;  // row of P or dS in LDS
+
+template <class T, int DP>
+constexpr size_t short_lds(size_t view, int buckets, bool table) {
+  const size_t sums = table ? ATT_WAVES * 256 * (size_t)buckets : 0, ps = (size_t)SHORT * PS * sizeof(T);
+  return 2 * short_tile<T, DP>() + 544 + view + (sums > ps ? sums : ps);
+}
+
+template <class T, int DP, bool GEN>
+__global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad_kernel(const AttArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  using M = Mma<T>;
+  const fx_attention& p = a.p;
+  constexpr int DB = DP / 32, ST = tile_stride<T>(DP);
+  T* const t0 = reinterpret_cast<T*>(smem);  // K, then the queries
+  T* const t1 = t0 + SHORT * ST;             // V, then the cotangent
+  unsigned char* rest = reinterpret_cast<unsigned char*>(t1 + SHORT * ST);
+  int* const kpos = reinterpret_cast<int*>(rest);
+  unsigned long long* const kok = reinterpret_cast<unsigned long long*>(rest + 512);
+  rest += 544;
+  BiasView bv;
+  bv.radius = p.radius;
+  bv.lut = reinterpret_cast<float*>(rest);
+  bv.map = rest + 4 * (GEN ? p.buckets : bias_entries(false, p.radius));
+  rest += view_lds(GEN, p.radius, p.buckets);
+  float* const ds_sums = reinterpret_cast<float*>(rest);  // [wave][bucket][64]
+  T* const ps = reinterpret_cast<T*>(rest);               // then [query][key]
+
+  const Place at(xcd_item(blockIdx.x, a.items), p.heads, 1);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int qi = 32 * wave + (lane & 31);
+  const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
+  const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
+  const bool in = qi < qlen;
+  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
+  const int64_t row = (at.b * p.nq + qi) * p.heads + at.h;
+
+  // K and V, 64 rows at a time
+  {
+    const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + at.h * p.kh;
+    const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + at.h * p.vh;
+    TileLoad<T, DP> kl[2], vl[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int k0 = i * ATT_TILE;
+      auto live = [&](int r) { return !GEN || !p.mask || p.mask[at.b * p.nk + k0 + r]; };
+      kl[i].fetch(kbase + (int64_t)k0 * p.kn, p.kn, klen - k0, p.dim, a.whole, live);
+      vl[i].fetch(vbase + (int64_t)k0 * p.vn, p.vn, klen - k0, p.dim, a.whole, live);
+    }
+    fill_bias<GEN>(p, at.h, bv, a.inv_scale);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      kl[i].put(t0 + i * ATT_TILE * ST);
+      vl[i].put(t1 + i * ATT_TILE * ST);
+    }
+    if (GEN && wave < 2) fill_keys(p, at.b, wave * ATT_TILE, klen, KeyView{kpos + wave * ATT_TILE, kok + wave}, lane);
+  }
+  Sums sums{ds_sums + wave * p.buckets * 64 + lane, nullptr, 0.0f, {}, {}};
+  if (p.grad_table)
+    for (int t = 0; t < p.buckets; ++t) sums.ds[64 * t] = 0.0f;
+  RowFrags<T, DP> q, g;
+  q.load(static_cast<const T*>(p.q) + at.b * p.qb + (int64_t)qi * p.qn + at.h * p.qh, in, p.dim, a.whole, half);
+  g.load(static_cast<const T*>(p.grad_out) + row * p.dim, in, p.dim, a.whole, half);
+  const float2 ml = in ? reinterpret_cast<const float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi]
+                       : make_float2(0.0f, INFINITY);
+  const float base = ml.x * a.c + ml.y;
+  const bool exact = __any(fabsf(ml.x * a.c) > BASE_MAX);
+  __syncthreads();
+
+  // P and dP of all keys, delta
+  const int64_t last = !in ? 0 : p.causal ? min((int64_t)klen, (int64_t)p.offset + qi + 1) : (int64_t)klen;
+  v16f s[4], dp[4];
+  float delta = 0.0f;
+  int far[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) far[i] = GEN ? 0 : far_side(i * ATT_TILE - (p.offset + 32 * wave), ATT_TILE, 32, p.radius);
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb) {
+    s[kb] = dp[kb] = v16f{};
+    if (32 * kb >= klen) continue;
+    const int k0 = kb / 2 * ATT_TILE;
+    const KeyView kv{kpos + k0, kok + kb / 2};
+    s[kb] = bias_block<GEN>(p, bv, kv, kb & 1, k0, qpos, half, far[kb / 2]);
+    s[kb] = row_product<T, DP>(t0, 32 * kb, q, s[kb], lane);
+    dp[kb] = row_product<T, DP>(t1, 32 * kb, g, dp[kb], lane);
+    if (exact) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i] - ml.x, a.c, -ml.y));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.c, -base));
+    }
+    const int left = (int)last - 32 * kb - 4 * half;
+    if (!__all(left >= 28)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = acc_row(i) < left ? s[kb][i] : 0.0f;
+    }
+    if (GEN && p.mask) {
+      const unsigned ok = (unsigned)(kok[kb / 2] >> (32 * (kb & 1))) >> (4 * half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = (ok >> acc_row(i)) & 1 ? s[kb][i] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) delta += s[kb][i] * dp[kb][i];
+  }
+  delta = half_sum(delta);
+
+  // dS, its bucket sums, dq; P and dS rounded for the second half
+  v16f dq[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dq[d] = v16f{};
+  typename M::frag pr[4][2], sr[4][2];
+#pragma unroll
+  for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pr[kb][i] = M::from_acc(s[kb], i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[kb][i] = s[kb][i] * (dp[kb][i] - delta);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sr[kb][i] = M::from_acc(dp[kb], i);
+    if (32 * kb >= klen) continue;
+    const int k0 = kb / 2 * ATT_TILE;
+    if (p.grad_table)
+      bucket_add<GEN, false>(bv, KeyView{kpos + k0, nullptr}, sums, dp[kb], s[kb], kb & 1, k0, qpos, half, far[kb / 2]);
+    column_product<T, DP>(t0, 32 * kb, dp[kb], dq, lane);
+  }
+  if (qi < p.nq) store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, dq, p.scale, p.dim, a.whole4, half);
+  if (!GEN && p.grad_table) add_pair(sums.ds, bv.map[0], sums.far_ds[0], bv.map[2 * p.radius + 128], sums.far_ds[1]);
+  __syncthreads();
+  if (p.grad_table) {
+    float* out = a.part + (at.h * p.batch + at.b) * p.buckets;
+    // four lanes a bucket, one for each wave's sums
+    for (int t = threadIdx.x / ATT_WAVES; t < p.buckets; t += ATT_NT / ATT_WAVES) {
+      const float* w = ds_sums + ((threadIdx.x % ATT_WAVES) * p.buckets + t) * 64;
+      float x = 0.0f;
+#pragma unroll 8
+      for (int l = 0; l < 64; ++l) x += w[(l + threadIdx.x) & 63];  // rotated: no shared bank
+      x = group_sum<ATT_WAVES>(x);
+      if (threadIdx.x % ATT_WAVES == 0) out[t] = x;
+    }
+  }
+
+  // the wave's rows of q and dO for K and V; P
+#pragma unroll
+  for (int i = 0; i < RowFrags<T, DP>::STEPS; ++i) {
+    const int o = qi * ST + M::KS * i + M::KS / 2 * half;
+    *reinterpret_cast<typename M::frag*>(t0 + o) = q.f[i];
+    *reinterpret_cast<typename M::frag*>(t1 + o) = g.f[i];
+  }
+  auto put = [&](const typename M::frag(&x)[4][2]) {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // registers 8 i ..: keys 16 i + 4 half + 0..3, then those 8 on
+        T* o = ps + qi * PS + 32 * kb + 16 * i + 4 * half;
+        *reinterpret_cast<vec_t<T, 4>*>(o) = __builtin_shufflevector(x[kb][i], x[kb][i], 0, 1, 2, 3);
+        *reinterpret_cast<vec_t<T, 4>*>(o + 8) = __builtin_shufflevector(x[kb][i], x[kb][i], 4, 5, 6, 7);
+      }
+  };
+  // rows: the tile's columns; columns: the wave's keys; contracted over the queries
+  auto over_queries = [&](const T* tile, v16f(&acc)[DB]) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = v16f{};
+#pragma unroll
+    for (int s = 0; s < SHORT / M::KS; ++s) {
+      if (M::KS * s >= qlen) break;
+      const typename M::frag b = M::columns(ps, PS, M::KS * s, 32 * wave, lane);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) acc[d] = M::mma(M::columns(tile, ST, M::KS * s, 32 * d, lane), b, acc[d]);
+    }
+  };
+  __syncthreads();  // the bucket sums have been read
+  put(pr);
+  __syncthreads();
+  v16f acc[DB];
+  const int ki = 32 * wave + (lane & 31);
+  const int64_t krow = ((at.b * p.nk + ki) * p.kv_heads + at.h) * p.dim;
+  over_queries(t1, acc);
+  __syncthreads();
+  put(sr);
+  if (ki < p.nk) store_rows<T, DP>(static_cast<T*>(p.grad_v) + krow, acc, 1.0f, p.dim, a.whole4, half);
+  __syncthreads();
+  over_queries(t0, acc);
+  if (ki < p.nk) store_rows<T, DP>(static_cast<T*>(p.grad_k) + krow, acc, p.scale, p.dim, a.whole4, half);
+}
+
+}  // namespace
+
+// Short sequences whose heads do not share K and V.
+bool attention_grad_short_fits(const fx_attention& p) {
+  return p.dtype != FX_F32 && p.nq >= 1 && p.nq <= SHORT && p.nk >= 1 && p.nk <= SHORT && p.heads == p.kv_heads;
+}
+
+int launch_attention_grad_short(const AttArgs& a, hipStream_t s) {
+  const fx_attention& p = a.p;
+  auto go = [&](auto t, auto dp, auto gen) {
+    using T = decltype(t);
+    constexpr int DP = decltype(dp)::value;
+    constexpr bool GEN = decltype(gen)::value != 0;
+    const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius, p.buckets), p.buckets, p.grad_table != nullptr);
+    hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds, s, a);
+  };
+  return attention_shape(p, [&](auto t, auto dp, auto gen) {
+    if constexpr (sizeof(t) == 2) go(t, dp, gen);
+  });
+}
+
+}  // namespace net
+}  // namespace fx
