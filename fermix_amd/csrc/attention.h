@@ -201,23 +201,42 @@ __device__ __forceinline__ float half_max(float x) { return join32<MaxOp>(x); }
 __device__ __forceinline__ float half_sum(float x) { return join32<AddOp>(x); }
 
 // A transposed accumulator (rows: 32 d + .. columns of the result; column: the lane's row) times f, as
-// rows of memory.
+// rows of memory, 16 bytes a store: the halves of a wave swap what they hold of two groups of eight columns.
+// Call with the whole wave; row and in are the lane's (both halves the same).
 template <class T, int DP>
-__device__ __forceinline__ void store_rows(T* row, const v16f (&acc)[DP / 32], float f, int dim, bool whole, int half) {
+__device__ __forceinline__ void store_rows(T* row, bool in, const v16f (&acc)[DP / 32], float f, int dim, bool whole,
+                                           int half) {
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int c = 32 * d + 8 * g + 4 * half;
-      vec_t<T, 4> x;
+    for (int g = 0; g < 4; g += 2) {
+      vec_t<T, 4> x[2];  // rounded in one place, so that the ways to store agree
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = (T)(acc[d][4 * g + r] * f);
-      if (whole) {
-        if (c < dim) *reinterpret_cast<vec_t<T, 4>*>(row + c) = x;
-      } else {
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (c + r < dim) row[c + r] = x[r];
+        for (int r = 0; r < 4; ++r) x[i][r] = (T)(acc[d][4 * (g + i) + r] * f);
+      if constexpr (sizeof(T) == 2) {
+        if (whole) {
+          typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+          const u32x2 y = __builtin_bit_cast(u32x2, x[0]), z = __builtin_bit_cast(u32x2, x[1]);
+          // lanes 0..31 get the even group's eight columns, 32..63 the odd one's
+          const auto a = __builtin_amdgcn_permlane32_swap(y[0], z[0], false, false);
+          const auto b = __builtin_amdgcn_permlane32_swap(y[1], z[1], false, false);
+          const int c = 32 * d + 8 * (g + half);
+          if (in && c < dim) *reinterpret_cast<uint4*>(row + c) = make_uint4(a[0], b[0], a[1], b[1]);
+          continue;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = 32 * d + 8 * (g + i) + 4 * half;
+        if (whole) {
+          if (in && c < dim) *reinterpret_cast<vec_t<T, 4>*>(row + c) = x[i];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (in && c + r < dim) row[c + r] = x[i][r];
+        }
       }
     }
 }
@@ -227,26 +246,40 @@ __device__ __forceinline__ void store_rows(T* row, const v16f (&acc)[DP / 32], f
 //    out over the distances -(R + 64) .. R + 64, saturated past R. A lane clamps once a tile, and
 //    the tile's values follow at constant offsets; a tile that lies past R as a whole has one value.
 //  - positions from memory (GEN = true): each pair's distance is clamped and looked up, map then table.
-struct BiasView {
-  float* lut;           // GEN: table [buckets]; else [2 R + 129] over distances
-  unsigned char* map;   // GEN: [2 R + 1]; else [2 R + 129] buckets over distances
-  int radius;
-};
+constexpr int MAX_BUCKETS = FX_MAX_ATTENTION_BUCKETS;
 __device__ __host__ constexpr int bias_entries(bool gen, int radius) { return gen ? 2 * radius + 1 : 2 * radius + 129; }
+struct BiasView {
+  float* table;        // [MAX_BUCKETS]
+  float* lut;          // (not GEN) [2 R + 129] over distances
+  unsigned char* map;  // GEN: [2 R + 1]; else [2 R + 129] buckets over distances
+  int radius;
+  __device__ __forceinline__ BiasView(bool gen, unsigned char* at, int r)
+      : table(reinterpret_cast<float*>(at)), lut(table + MAX_BUCKETS),
+        map(at + 4 * (MAX_BUCKETS + (gen ? 0 : bias_entries(false, r)))), radius(r) {}
+};
+// Bytes of a BiasView.
+constexpr size_t view_lds(bool gen, int radius) {
+  return (4 * (size_t)(MAX_BUCKETS + (gen ? 0 : bias_entries(false, radius))) + bias_entries(gen, radius) + 15) / 16 * 16;
+}
 
-// Fills the view; `head` of the table (NULL: no bias). All threads of the workgroup; a barrier follows.
+// Fills the view from `head` of the table (NULL: no bias) in two steps, so that the loads are all on their way at
+// once: load (from memory; a barrier follows), lay (within LDS; a barrier follows). All threads.
 template <bool GEN>
-__device__ __forceinline__ void fill_bias(const fx_attention& p, int head, const BiasView& b, float inv_scale) {
+__device__ __forceinline__ void load_bias(const fx_attention& p, int head, const BiasView& b, float inv_scale) {
+  float x = 0.0f;
+  if (p.table && (int)threadIdx.x < p.buckets)
+    x = scaled_bias(p.table[(int64_t)threadIdx.x * p.heads + head], inv_scale);
   const int n = bias_entries(GEN, b.radius);
   for (int i = threadIdx.x; i < n; i += ATT_NT) {
     const int d = GEN ? i : max(0, min(2 * b.radius, i - 64));
-    const int t = p.table ? min((int)p.map[d], p.buckets - 1) : 0;
-    b.map[i] = (unsigned char)t;
-    if constexpr (!GEN) b.lut[i] = p.table ? scaled_bias(p.table[(int64_t)t * p.heads + head], inv_scale) : 0.0f;
+    b.map[i] = p.table ? (unsigned char)min((int)p.map[d], p.buckets - 1) : 0;
   }
-  if constexpr (GEN)
-    for (int i = threadIdx.x; i < p.buckets; i += ATT_NT)
-      b.lut[i] = p.table ? scaled_bias(p.table[(int64_t)i * p.heads + head], inv_scale) : 0.0f;
+  if ((int)threadIdx.x < MAX_BUCKETS) b.table[threadIdx.x] = x;
+}
+template <bool GEN>
+__device__ __forceinline__ void lay_bias(const BiasView& b) {
+  if constexpr (!GEN)
+    for (int i = threadIdx.x; i < bias_entries(false, b.radius); i += ATT_NT) b.lut[i] = b.table[b.map[i]];
 }
 
 // A workgroup's place: items are laid out so that those of one kv head follow each other, and each of
@@ -260,7 +293,6 @@ __device__ __forceinline__ int64_t xcd_item(int64_t block, int64_t total) {
 struct AttArgs {
   fx_attention p;
   int whole;   // rows are whole 16-byte vectors
-  int whole4;  // result rows are whole vectors of four elements
   float c;     // scale log2(e)
   float inv_scale;
   int tiles;   // items of a head
@@ -320,7 +352,7 @@ __device__ __forceinline__ v16f bias_block(const fx_attention& p, const BiasView
       const int k[4] = {kp.x, kp.y, kp.z, kp.w};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[4 * g + r] = bv.lut[distance_bucket(bv.map, bv.radius, k[r], qpos)];
+        x[4 * g + r] = bv.table[distance_bucket(bv.map, bv.radius, k[r], qpos)];
       }
     }
   } else {
@@ -356,11 +388,6 @@ int attention_shape(const fx_attention& p, F&& f) {
 }
 
 // ------------------------------------------------------------------ gradient
-
-// Bytes of a BiasView.
-constexpr size_t view_lds(bool gen, int radius, int buckets) {
-  return ((gen ? 4 * (size_t)buckets : 4 * (size_t)bias_entries(false, radius)) + bias_entries(gen, radius) + 15) / 16 * 16;
-}
 
 // The lane's bucket sums: of dS, of its query's P (WEIGHTS: the 16-bit types), and what tiles past the
 // radius add to the first and the last distance's bucket.

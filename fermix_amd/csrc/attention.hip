@@ -12,9 +12,8 @@ namespace net {
 namespace {
 
 template <class T, int DP>
-constexpr size_t forward_lds(bool gen, int radius, int buckets) {
-  return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T) + (gen ? 272 + 4 * buckets : 4 * bias_entries(false, radius)) +
-         bias_entries(gen, radius);
+constexpr size_t forward_lds(bool gen, int radius) {
+  return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T) + (gen ? 272 : 0) + view_lds(gen, radius);
 }
 
 template <class T, int DP, bool GEN>
@@ -27,10 +26,7 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
   unsigned char* rest = reinterpret_cast<unsigned char*>(vt + TS);
   KeyView kv{reinterpret_cast<int*>(rest), reinterpret_cast<unsigned long long*>(rest + 256)};
   if (GEN) rest += 272;
-  BiasView bv;
-  bv.radius = p.radius;
-  bv.lut = reinterpret_cast<float*>(rest);
-  bv.map = rest + 4 * (GEN ? p.buckets : bias_entries(false, p.radius));
+  const BiasView bv(GEN, rest, p.radius);
 
   const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -46,7 +42,6 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
   const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + kh * p.kh;
   const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + kh * p.vh;
 
-  fill_bias<GEN>(p, at.h, bv, a.inv_scale);
   RowFrags<T, DP> q;
   q.load(static_cast<const T*>(p.q) + at.b * p.qb + (int64_t)qi * p.qn + at.h * p.qh, in, p.dim, a.whole, half);
   v16f o[DB];
@@ -61,6 +56,9 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
     vl.fetch(vbase + (int64_t)k0 * p.vn, p.vn, keys - k0, p.dim, a.whole, live);
   };
   if (keys > 0) fetch(0);
+  load_bias<GEN>(p, at.h, bv, a.inv_scale);
+  __syncthreads();
+  lay_bias<GEN>(bv);
   // last key that some query of the wave can see
   const int64_t wave_last = p.causal ? (int64_t)p.offset + q0 + 32 * wave + 31 : (int64_t)p.nk;
   for (int k0 = 0; k0 < keys; k0 += ATT_TILE) {
@@ -118,12 +116,12 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
     for (int kb = 0; kb < 2; ++kb) column_product<T, DP>(vt, 32 * kb, s[kb], o, lane);
   }
 
-  if (qi >= p.nq) return;
+  const bool out_in = qi < p.nq;
   l = half_sum(l);
   const float inv = l > 0.0f ? 1.0f / l : (l != l ? l : 0.0f);
   const int64_t row = (at.b * p.nq + qi) * p.heads + at.h;
-  store_rows<T, DP>(static_cast<T*>(p.out) + row * p.dim, o, inv, p.dim, a.whole4, half);
-  if (p.stats && half == 0)
+  store_rows<T, DP>(static_cast<T*>(p.out) + row * p.dim, out_in, o, inv, p.dim, a.whole, half);
+  if (p.stats && out_in && half == 0)
     reinterpret_cast<float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi] =
         l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
 }
@@ -162,7 +160,6 @@ AttArgs attention_args(const fx_attention& p) {
   const uintptr_t in = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.grad_out | (uintptr_t)p.out |
                        (uintptr_t)p.grad_q | (uintptr_t)p.grad_k | (uintptr_t)p.grad_v;
   a.whole = strides % v == 0 && !(in & 15);
-  a.whole4 = p.dim % 4 == 0 && !(in & 15);
   a.c = p.scale * LOG2E;
   a.inv_scale = 1.0f / p.scale;
   return a;
@@ -186,7 +183,7 @@ extern "C" int fx_attention_forward(const fx_attention* p, fx_stream_t stream) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
-    const size_t lds = forward_lds<T, DP>(GEN, p->radius, p->buckets);
+    const size_t lds = forward_lds<T, DP>(GEN, p->radius);
     hipLaunchKernelGGL((attention_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds, (hipStream_t)stream,
                        a);
   });

@@ -34,12 +34,9 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   unsigned char* rest = reinterpret_cast<unsigned char*>(vt + TS);
   KeyView kv{reinterpret_cast<int*>(rest), reinterpret_cast<unsigned long long*>(rest + 256)};
   rest += 272;
-  BiasView bv;
-  bv.radius = p.radius;
-  bv.lut = reinterpret_cast<float*>(rest);
-  bv.map = rest + 4 * (GEN ? p.buckets : bias_entries(false, p.radius));
+  const BiasView bv(GEN, rest, p.radius);
   constexpr bool WEIGHTS = sizeof(T) == 2;
-  float* const row_sum = reinterpret_cast<float*>(rest + view_lds(GEN, p.radius, p.buckets));  // [wave][32]
+  float* const row_sum = reinterpret_cast<float*>(rest + view_lds(GEN, p.radius));  // [wave][32]
   float* const ds_sums = row_sum + 32 * ATT_WAVES;                                             // [wave][bucket][64]
   unsigned* const weights = reinterpret_cast<unsigned*>(ds_sums + 64 * ATT_WAVES * p.buckets);  // [wave][bucket][32]
 
@@ -57,7 +54,6 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + kh * p.vh;
   const int64_t row = (at.b * p.nq + qi) * p.heads + at.h, stat = (at.b * p.heads + at.h) * p.nq + qi;
 
-  fill_bias<GEN>(p, at.h, bv, a.inv_scale);
   Sums sums{ds_sums + wave * p.buckets * 64 + lane, weights + wave * p.buckets * 32 + (lane & 31), 0.0f, {}, {}};
   if (p.grad_table)
     for (int t = 0; t < p.buckets; ++t) {
@@ -91,6 +87,9 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
     vl.fetch(vbase + (int64_t)k0 * p.vn, p.vn, keys - k0, p.dim, a.whole, live);
   };
   if (keys > 0) fetch(0);
+  load_bias<GEN>(p, at.h, bv, a.inv_scale);
+  __syncthreads();
+  lay_bias<GEN>(bv);
   const int64_t wave_last = p.causal ? (int64_t)p.offset + q0 + 32 * wave + 31 : (int64_t)p.nk;
   for (int k0 = 0; k0 < keys; k0 += ATT_TILE) {
     __syncthreads();
@@ -136,8 +135,7 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
       column_product<T, DP>(kt, 32 * kb, dp, dq, lane);
     }
   }
-  if (qi < p.nq)
-    store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, dq, p.scale, p.dim, a.whole4, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
   // what dS add up to is delta's error (WEIGHTS): the second launch gets delta without it
   const float all = WEIGHTS ? half_sum(sums.all) : 0.0f;
   if (qi < p.nq && half == 0) a.delta[stat] = delta + all;
@@ -189,7 +187,7 @@ __device__ __forceinline__ v16f bias_block_t(const BiasView& bv, const QueryView
       const int q[4] = {qp.x, qp.y, qp.z, qp.w};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[4 * g + r] = bv.lut[distance_bucket(bv.map, bv.radius, kpos, q[r])];
+        x[4 * g + r] = bv.table[distance_bucket(bv.map, bv.radius, kpos, q[r])];
       }
     }
   } else {
@@ -212,10 +210,7 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   float* const f = reinterpret_cast<float*>(rest);
   QueryView qv{reinterpret_cast<int*>(rest), f + 64, f + 128, f + 192, reinterpret_cast<unsigned*>(f + 256)};
   rest += 1040;
-  BiasView bv;
-  bv.radius = p.radius;
-  bv.lut = reinterpret_cast<float*>(rest);
-  bv.map = rest + 4 * (GEN ? p.buckets : bias_entries(false, p.radius));
+  const BiasView bv(GEN, rest, p.radius);
 
   const Place at(xcd_item(blockIdx.x, a.items), p.kv_heads, a.tiles);  // heads: those of k and v
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -241,8 +236,6 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
     const T* qbase = static_cast<const T*>(p.q) + at.b * p.qb + h * p.qh;
     const T* gbase = static_cast<const T*>(p.grad_out) + (at.b * p.nq * p.heads + h) * p.dim;
     const int64_t stat = (at.b * p.heads + h) * p.nq;
-    __syncthreads();
-    fill_bias<GEN>(p, h, bv, a.inv_scale);
     TileLoad<T, DP> ql, gl;
     auto fetch = [&](int q0) {
       auto live = [](int) { return true; };
@@ -250,6 +243,10 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
       gl.fetch(gbase + (int64_t)q0 * p.heads * p.dim, (int64_t)p.heads * p.dim, queries - q0, p.dim, a.whole, live);
     };
     if (first < queries) fetch(first);
+    __syncthreads();  // the last head's view has been read
+    load_bias<GEN>(p, h, bv, a.inv_scale);
+    __syncthreads();
+    lay_bias<GEN>(bv);
     for (int q0 = first; q0 < queries; q0 += ATT_TILE) {
       __syncthreads();
       ql.put(qt);
@@ -312,10 +309,9 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
       }
     }
   }
-  if (ki >= p.nk) return;
   const int64_t row = ((at.b * p.nk + ki) * p.kv_heads + at.h) * p.dim;
-  store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, dk, p.scale, p.dim, a.whole4, half);
-  store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, dv, 1.0f, p.dim, a.whole4, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, dk, p.scale, p.dim, a.whole, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, dv, 1.0f, p.dim, a.whole, half);
 }
 
 int64_t delta_floats(const fx_attention& p) { return cdiv(p.batch * p.heads * p.nq, 4) * 4; }
@@ -367,7 +363,7 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
-    const size_t tiles = tiles_lds<T, DP>(), view = view_lds(GEN, p->radius, p->buckets);
+    const size_t tiles = tiles_lds<T, DP>(), view = view_lds(GEN, p->radius);
     const size_t sums = ATT_WAVES * (128 + (sizeof(T) == 2 ? 384 : 256) * (size_t)p->buckets);
     const size_t lds_q = tiles + 272 + view + (p->grad_table ? sums : 0);
     const size_t lds_kv = tiles + 1040 + view;

@@ -38,11 +38,8 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   int* const kpos = reinterpret_cast<int*>(rest);
   unsigned long long* const kok = reinterpret_cast<unsigned long long*>(rest + 512);
   rest += 544;
-  BiasView bv;
-  bv.radius = p.radius;
-  bv.lut = reinterpret_cast<float*>(rest);
-  bv.map = rest + 4 * (GEN ? p.buckets : bias_entries(false, p.radius));
-  rest += view_lds(GEN, p.radius, p.buckets);
+  const BiasView bv(GEN, rest, p.radius);
+  rest += view_lds(GEN, p.radius);
   float* const ds_sums = reinterpret_cast<float*>(rest);  // [wave][bucket][64]
   T* const ps = reinterpret_cast<T*>(rest);               // then [query][key]
 
@@ -55,7 +52,8 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
   const int64_t row = (at.b * p.nq + qi) * p.heads + at.h;
 
-  // K and V, 64 rows at a time
+  // K and V, 64 rows at a time, and the wave's own rows
+  RowFrags<T, DP> q, g;
   {
     const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + at.h * p.kh;
     const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + at.h * p.vh;
@@ -67,7 +65,9 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
       kl[i].fetch(kbase + (int64_t)k0 * p.kn, p.kn, klen - k0, p.dim, a.whole, live);
       vl[i].fetch(vbase + (int64_t)k0 * p.vn, p.vn, klen - k0, p.dim, a.whole, live);
     }
-    fill_bias<GEN>(p, at.h, bv, a.inv_scale);
+    q.load(static_cast<const T*>(p.q) + at.b * p.qb + (int64_t)qi * p.qn + at.h * p.qh, in, p.dim, a.whole, half);
+    g.load(static_cast<const T*>(p.grad_out) + row * p.dim, in, p.dim, a.whole, half);
+    load_bias<GEN>(p, at.h, bv, a.inv_scale);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       kl[i].put(t0 + i * ATT_TILE * ST);
@@ -78,14 +78,15 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   Sums sums{ds_sums + wave * p.buckets * 64 + lane, nullptr, 0.0f, {}, {}};
   if (p.grad_table)
     for (int t = 0; t < p.buckets; ++t) sums.ds[64 * t] = 0.0f;
-  RowFrags<T, DP> q, g;
-  q.load(static_cast<const T*>(p.q) + at.b * p.qb + (int64_t)qi * p.qn + at.h * p.qh, in, p.dim, a.whole, half);
-  g.load(static_cast<const T*>(p.grad_out) + row * p.dim, in, p.dim, a.whole, half);
   const float2 ml = in ? reinterpret_cast<const float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi]
                        : make_float2(0.0f, INFINITY);
   const float base = ml.x * a.c + ml.y;
   const bool exact = __any(fabsf(ml.x * a.c) > BASE_MAX);
   __syncthreads();
+  if (!GEN) {
+    lay_bias<GEN>(bv);
+    __syncthreads();
+  }
 
   // P and dP of all keys, delta
   const int64_t last = !in ? 0 : p.causal ? min((int64_t)klen, (int64_t)p.offset + qi + 1) : (int64_t)klen;
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
       bucket_add<GEN, false>(bv, KeyView{kpos + k0, nullptr}, sums, dp[kb], s[kb], kb & 1, k0, qpos, half, far[kb / 2]);
     column_product<T, DP>(t0, 32 * kb, dp[kb], dq, lane);
   }
-  if (qi < p.nq) store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, dq, p.scale, p.dim, a.whole4, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
   if (!GEN && p.grad_table) add_pair(sums.ds, bv.map[0], sums.far_ds[0], bv.map[2 * p.radius + 128], sums.far_ds[1]);
   __syncthreads();
   if (p.grad_table) {
@@ -199,10 +200,10 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   over_queries(t1, acc);
   __syncthreads();
   put(sr);
-  if (ki < p.nk) store_rows<T, DP>(static_cast<T*>(p.grad_v) + krow, acc, 1.0f, p.dim, a.whole4, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_v) + krow, ki < p.nk, acc, 1.0f, p.dim, a.whole, half);
   __syncthreads();
   over_queries(t0, acc);
-  if (ki < p.nk) store_rows<T, DP>(static_cast<T*>(p.grad_k) + krow, acc, p.scale, p.dim, a.whole4, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_k) + krow, ki < p.nk, acc, p.scale, p.dim, a.whole, half);
 }
 
 }  // namespace
@@ -218,7 +219,7 @@ int launch_attention_grad_short(const AttArgs& a, hipStream_t s) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
-    const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius, p.buckets), p.buckets, p.grad_table != nullptr);
+    const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius), p.buckets, p.grad_table != nullptr);
     hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds, s, a);
   };
   return attention_shape(p, [&](auto t, auto dp, auto gen) {
