@@ -103,7 +103,6 @@ __device__ __forceinline__ void exp_block(v16f& s, float c, float m, float base,
   }
 }
 
-constexpr int ATT_WAVES = 4, ATT_NT = 64 * ATT_WAVES;
 constexpr int ATT_TILE = 64;  // rows of a staged tile
 
 template <class T>
@@ -114,17 +113,17 @@ constexpr int tile_stride(int dp) {
 // A tile of up to 64 rows of dim elements, through registers into LDS: fetch starts the loads, put
 // stores them. Rows at or past `rows`, and those that `live` refuses, become zero, so that nothing a
 // masked row holds enters a product; columns dim .. DP too.
-template <class T, int DP>
+template <class T, int DP, int NT>
 struct TileLoad {
-  static constexpr int V = VEC16<T>, CHUNKS = DP / V, PER = ATT_TILE * CHUNKS / ATT_NT;
-  static_assert(PER >= 1 && PER * ATT_NT == ATT_TILE * CHUNKS, "whole turns");
+  static constexpr int V = VEC16<T>, CHUNKS = DP / V, PER = ATT_TILE * CHUNKS / NT;
+  static_assert(PER >= 1 && PER * NT == ATT_TILE * CHUNKS, "whole turns");
   vec_t<T, V> x[PER];
 
   template <class L>
   __device__ __forceinline__ void fetch(const T* base, int64_t row_stride, int rows, int dim, bool whole, L&& live) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = i * ATT_NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
+      const int at = i * NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
       x[i] = {};
       if (r < rows && c < dim && live(r)) {
         const T* p = base + r * row_stride + c;
@@ -141,7 +140,7 @@ struct TileLoad {
   __device__ __forceinline__ void put(T* tile) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = i * ATT_NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
+      const int at = i * NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
       *reinterpret_cast<vec_t<T, V>*>(tile + r * tile_stride<T>(DP) + c) = x[i];
     }
   }
@@ -264,22 +263,22 @@ constexpr size_t view_lds(bool gen, int radius) {
 
 // Fills the view from `head` of the table (NULL: no bias) in two steps, so that the loads are all on their way at
 // once: load (from memory; a barrier follows), lay (within LDS; a barrier follows). All threads.
-template <bool GEN>
+template <bool GEN, int NT>
 __device__ __forceinline__ void load_bias(const fx_attention& p, int head, const BiasView& b, float inv_scale) {
   float x = 0.0f;
   if (p.table && (int)threadIdx.x < p.buckets)
     x = scaled_bias(p.table[(int64_t)threadIdx.x * p.heads + head], inv_scale);
   const int n = bias_entries(GEN, b.radius);
-  for (int i = threadIdx.x; i < n; i += ATT_NT) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const int d = GEN ? i : max(0, min(2 * b.radius, i - 64));
     b.map[i] = p.table ? (unsigned char)min((int)p.map[d], p.buckets - 1) : 0;
   }
   if ((int)threadIdx.x < MAX_BUCKETS) b.table[threadIdx.x] = x;
 }
-template <bool GEN>
+template <bool GEN, int NT>
 __device__ __forceinline__ void lay_bias(const BiasView& b) {
   if constexpr (!GEN)
-    for (int i = threadIdx.x; i < bias_entries(false, b.radius); i += ATT_NT) b.lut[i] = b.table[b.map[i]];
+    for (int i = threadIdx.x; i < bias_entries(false, b.radius); i += NT) b.lut[i] = b.table[b.map[i]];
 }
 
 // A workgroup's place: items are laid out so that those of one kv head follow each other, and each of
@@ -301,14 +300,15 @@ struct AttArgs {
   float* part;   // gradient: bucket sums [head][batch * tiles][buckets]
 };
 
-// An item's place: sample, head and tile. Within a head the last tile comes first (with causal it has the
-// most keys), the heads that share K and V follow each other.
+// An item's place: sample, head and tile. The heads that share K and V follow each other; within a head the tile with
+// the most work under causal comes first: the last of the queries (last_first), the first of the keys.
 struct Place {
   int64_t b;
   int h, tile;
-  __device__ __forceinline__ Place(int64_t item, int heads, int tiles) {
+  __device__ __forceinline__ Place(int64_t item, int heads, int tiles, bool last_first) {
     const int64_t bh = item / tiles;
-    tile = tiles - 1 - (int)(item - bh * tiles);
+    tile = (int)(item - bh * tiles);
+    if (last_first) tile = tiles - 1 - tile;
     b = bh / heads;
     h = (int)(bh - b * heads);
   }

@@ -16,8 +16,11 @@ constexpr size_t forward_lds(bool gen, int radius) {
   return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T) + (gen ? 272 : 0) + view_lds(gen, radius);
 }
 
-template <class T, int DP, bool GEN>
-__global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
+// WAVES: of a workgroup. Two waves a SIMD hide each other's waits (head dimension 128: 1411 -> 820 us at
+// 2 x 16 x 8192 queries); float32 rows of 128 do not fit their registers then.
+template <class T, int DP, bool GEN, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) void attention_kernel(const AttArgs a) {
+  constexpr int NT = 64 * WAVES;
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention& p = a.p;
   constexpr int DB = DP / 32, TS = ATT_TILE * tile_stride<T>(DP);
@@ -28,16 +31,16 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
   if (GEN) rest += 272;
   const BiasView bv(GEN, rest, p.radius);
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles);
+  const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles, true);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int q0 = at.tile * 32 * ATT_WAVES, qi = q0 + 32 * wave + (lane & 31);
+  const int q0 = at.tile * 32 * WAVES, qi = q0 + 32 * wave + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
   const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
   const bool in = qi < qlen;
   const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
   // keys that any query of the workgroup can see
   int keys = q0 < qlen ? klen : 0;
-  if (p.causal) keys = (int)min((int64_t)keys, (int64_t)p.offset + min(q0 + 32 * ATT_WAVES, qlen));
+  if (p.causal) keys = (int)min((int64_t)keys, (int64_t)p.offset + min(q0 + 32 * WAVES, qlen));
   const int kh = at.h / (p.heads / p.kv_heads);
   const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + kh * p.kh;
   const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + kh * p.vh;
@@ -49,16 +52,16 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
   for (int d = 0; d < DB; ++d) o[d] = v16f{};
   float m = -INFINITY, m_base = -INFINITY, l = 0.0f;  // maximum of the raw scores, that times c, sum
 
-  TileLoad<T, DP> kl, vl;
+  TileLoad<T, DP, NT> kl, vl;
   auto fetch = [&](int k0) {
     auto live = [&](int r) { return !GEN || !p.mask || p.mask[at.b * p.nk + k0 + r]; };
     kl.fetch(kbase + (int64_t)k0 * p.kn, p.kn, keys - k0, p.dim, a.whole, live);
     vl.fetch(vbase + (int64_t)k0 * p.vn, p.vn, keys - k0, p.dim, a.whole, live);
   };
   if (keys > 0) fetch(0);
-  load_bias<GEN>(p, at.h, bv, a.inv_scale);
+  load_bias<GEN, NT>(p, at.h, bv, a.inv_scale);
   __syncthreads();
-  lay_bias<GEN>(bv);
+  lay_bias<GEN, NT>(bv);
   // last key that some query of the wave can see
   const int64_t wave_last = p.causal ? (int64_t)p.offset + q0 + 32 * wave + 31 : (int64_t)p.nk;
   for (int k0 = 0; k0 < keys; k0 += ATT_TILE) {
@@ -126,6 +129,8 @@ __global__ __launch_bounds__(ATT_NT) void attention_kernel(const AttArgs a) {
         l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
 }
 
+int forward_waves(const fx_attention& p) { return p.dim > 64 && p.dtype != FX_F32 && p.nq > 128 ? 8 : 4; }
+
 }  // namespace
 
 bool attention_sizes_ok(const fx_attention* p) {
@@ -176,7 +181,8 @@ extern "C" int fx_attention_forward(const fx_attention* p, fx_stream_t stream) {
   if (p->batch == 0 || p->nq == 0) return FX_OK;
   if (!attention_pointers_ok(*p)) return FX_ERR_INVALID_ARGUMENT;
   AttArgs a = attention_args(*p);
-  a.tiles = (int)cdiv(p->nq, 32 * ATT_WAVES);
+  const int waves = forward_waves(*p);
+  a.tiles = (int)cdiv(p->nq, 32 * waves);
   a.items = p->batch * p->heads * a.tiles;
   if (a.items > 0x7fffffff) return FX_ERR_UNSUPPORTED;
   return attention_shape(*p, [&](auto t, auto dp, auto gen) {
@@ -184,7 +190,13 @@ extern "C" int fx_attention_forward(const fx_attention* p, fx_stream_t stream) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
     const size_t lds = forward_lds<T, DP>(GEN, p->radius);
-    hipLaunchKernelGGL((attention_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds, (hipStream_t)stream,
-                       a);
+    auto go = [&](auto w) {
+      constexpr int WAVES = decltype(w)::value;
+      hipLaunchKernelGGL((attention_kernel<T, DP, GEN, WAVES>), dim3((unsigned)a.items), dim3(64 * WAVES), lds,
+                         (hipStream_t)stream, a);
+    };
+    if constexpr (DP == 128 && sizeof(T) == 2)
+      if (waves == 8) return go(ic<8>{});
+    go(ic<4>{});
   });
 }

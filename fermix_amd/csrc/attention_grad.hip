@@ -23,8 +23,11 @@ template <class T, int DP>
 constexpr size_t tiles_lds() {
   return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T);
 }
-template <class T, int DP, bool GEN>
-__global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void attention_dq_kernel(const AttArgs a) {
+// WAVES: of a workgroup.
+template <class T, int DP, bool GEN, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 128 || WAVES == 8 ? 2 : 1) void attention_dq_kernel(
+    const AttArgs a) {
+  constexpr int NT = 64 * WAVES;
   extern __shared__ __align__(16) unsigned char smem[];
   using M = Mma<T>;
   const fx_attention& p = a.p;
@@ -37,18 +40,18 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   const BiasView bv(GEN, rest, p.radius);
   constexpr bool WEIGHTS = sizeof(T) == 2;
   float* const row_sum = reinterpret_cast<float*>(rest + view_lds(GEN, p.radius));  // [wave][32]
-  float* const ds_sums = row_sum + 32 * ATT_WAVES;                                             // [wave][bucket][64]
-  unsigned* const weights = reinterpret_cast<unsigned*>(ds_sums + 64 * ATT_WAVES * p.buckets);  // [wave][bucket][32]
+  float* const ds_sums = row_sum + 32 * WAVES;                                             // [wave][bucket][64]
+  unsigned* const weights = reinterpret_cast<unsigned*>(ds_sums + 64 * WAVES * p.buckets);  // [wave][bucket][32]
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles);
+  const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles, true);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int q0 = at.tile * 32 * ATT_WAVES, qi = q0 + 32 * wave + (lane & 31);
+  const int q0 = at.tile * 32 * WAVES, qi = q0 + 32 * wave + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
   const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
   const bool in = qi < qlen;
   const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
   int keys = q0 < qlen ? klen : 0;
-  if (p.causal) keys = (int)min((int64_t)keys, (int64_t)p.offset + min(q0 + 32 * ATT_WAVES, qlen));
+  if (p.causal) keys = (int)min((int64_t)keys, (int64_t)p.offset + min(q0 + 32 * WAVES, qlen));
   const int kh = at.h / (p.heads / p.kv_heads);
   const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + kh * p.kh;
   const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + kh * p.vh;
@@ -80,16 +83,16 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   v16f dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = v16f{};
-  TileLoad<T, DP> kl, vl;
+  TileLoad<T, DP, NT> kl, vl;
   auto fetch = [&](int k0) {
     auto live = [&](int r) { return !GEN || !p.mask || p.mask[at.b * p.nk + k0 + r]; };
     kl.fetch(kbase + (int64_t)k0 * p.kn, p.kn, keys - k0, p.dim, a.whole, live);
     vl.fetch(vbase + (int64_t)k0 * p.vn, p.vn, keys - k0, p.dim, a.whole, live);
   };
   if (keys > 0) fetch(0);
-  load_bias<GEN>(p, at.h, bv, a.inv_scale);
+  load_bias<GEN, NT>(p, at.h, bv, a.inv_scale);
   __syncthreads();
-  lay_bias<GEN>(bv);
+  lay_bias<GEN, NT>(bv);
   const int64_t wave_last = p.causal ? (int64_t)p.offset + q0 + 32 * wave + 31 : (int64_t)p.nk;
   for (int k0 = 0; k0 < keys; k0 += ATT_TILE) {
     __syncthreads();
@@ -148,9 +151,9 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
     if (half == 0) row_sum[32 * wave + lane] = all;
     __syncthreads();
     float* out = a.part + ((at.h * p.batch + at.b) * a.tiles + at.tile) * p.buckets;
-    for (int t = threadIdx.x; t < p.buckets; t += ATT_NT) {
+    for (int t = threadIdx.x; t < p.buckets; t += NT) {
       float x = 0.0f, y = 0.0f;
-      for (int w = 0; w < ATT_WAVES; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
 #pragma unroll 4
         for (int l = 0; l < 64; ++l) x += ds_sums[(w * p.buckets + t) * 64 + ((l + t) & 63)];  // rotated: no shared bank
         if (WEIGHTS)
@@ -199,8 +202,13 @@ __device__ __forceinline__ v16f bias_block_t(const BiasView& bv, const QueryView
   return x;
 }
 
-template <class T, int DP, bool GEN>
-__global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void attention_dkv_kernel(const AttArgs a) {
+// Four waves have 32 keys each. SPLIT: eight do, the first four for dv and the others for dk of the same keys; both
+// form the scores (five products for four), but neither has to hold the other's sums, so that two waves fit a
+// SIMD where the rows are long.
+template <class T, int DP, bool GEN, bool SPLIT>
+__global__ __launch_bounds__(SPLIT ? 512 : 256, DP * (int)sizeof(T) <= 128 || SPLIT ? 2 : 1) void attention_dkv_kernel(
+    const AttArgs a) {
+  constexpr int NT = SPLIT ? 512 : 256;
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention& p = a.p;
   constexpr int DB = DP / 32, TS = ATT_TILE * tile_stride<T>(DP);
@@ -212,9 +220,10 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   rest += 1040;
   const BiasView bv(GEN, rest, p.radius);
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.kv_heads, a.tiles);  // heads: those of k and v
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int k0 = at.tile * 32 * ATT_WAVES, kw = k0 + 32 * wave, ki = kw + (lane & 31);
+  const Place at(xcd_item(blockIdx.x, a.items), p.kv_heads, a.tiles, false);  // heads: those of k and v
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, half = lane >> 5;
+  const bool do_v = !SPLIT || threadIdx.x < 256, do_k = !SPLIT || threadIdx.x >= 256;
+  const int k0 = at.tile * 128, kw = k0 + 32 * wave, ki = kw + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
   const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
   const bool in = ki < klen && !(GEN && p.mask && !p.mask[at.b * p.nk + ki]);
@@ -222,11 +231,14 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
   const int group = p.heads / p.kv_heads;
   RowFrags<T, DP> k, v;
   k.load(static_cast<const T*>(p.k) + at.b * p.kb + (int64_t)ki * p.kn + at.h * p.kh, in, p.dim, a.whole, half);
-  v.load(static_cast<const T*>(p.v) + at.b * p.vb + (int64_t)ki * p.vn + at.h * p.vh, in, p.dim, a.whole, half);
+  v.load(static_cast<const T*>(p.v) + at.b * p.vb + (int64_t)ki * p.vn + at.h * p.vh, in && do_k, p.dim, a.whole, half);
   const bool whole = __all(in);  // every lane's key is left
-  v16f dk[DB], dv[DB];
+  v16f sum[SPLIT ? 1 : 2][DB];   // dk (SPLIT: or dv), dv
 #pragma unroll
-  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = v16f{};
+  for (int d = 0; d < DB; ++d) {
+    sum[0][d] = v16f{};
+    if (!SPLIT) sum[SPLIT ? 0 : 1][d] = v16f{};
+  }
   // queries that some key of the workgroup is seen by
   const int first = p.causal ? max(0, k0 - p.offset) / ATT_TILE * ATT_TILE : 0;
   const int queries = k0 < klen ? qlen : 0;
@@ -236,7 +248,7 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
     const T* qbase = static_cast<const T*>(p.q) + at.b * p.qb + h * p.qh;
     const T* gbase = static_cast<const T*>(p.grad_out) + (at.b * p.nq * p.heads + h) * p.dim;
     const int64_t stat = (at.b * p.heads + h) * p.nq;
-    TileLoad<T, DP> ql, gl;
+    TileLoad<T, DP, NT> ql, gl;
     auto fetch = [&](int q0) {
       auto live = [](int) { return true; };
       ql.fetch(qbase + (int64_t)q0 * p.qn, p.qn, queries - q0, p.dim, a.whole, live);
@@ -244,9 +256,9 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
     };
     if (first < queries) fetch(first);
     __syncthreads();  // the last head's view has been read
-    load_bias<GEN>(p, h, bv, a.inv_scale);
+    load_bias<GEN, NT>(p, h, bv, a.inv_scale);
     __syncthreads();
-    lay_bias<GEN>(bv);
+    lay_bias<GEN, NT>(bv);
     for (int q0 = first; q0 < queries; q0 += ATT_TILE) {
       __syncthreads();
       ql.put(qt);
@@ -274,7 +286,6 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
       for (int qb = 0; qb < 2; ++qb) {
         v16f s = bias_block_t<GEN>(bv, qv, qb, p.offset + q0, kpos, half, far);
         s = row_product<T, DP>(qt, 32 * qb, k, s, lane);
-        v16f dp = row_product<T, DP>(gt, 32 * qb, v, v16f{}, lane);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int at4 = 32 * qb + 8 * g + 4 * half;
@@ -297,7 +308,9 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = in ? s[i] : 0.0f;
         }
-        column_product<T, DP>(gt, 32 * qb, s, dv, lane);
+        if (do_v) column_product<T, DP>(gt, 32 * qb, s, sum[SPLIT ? 0 : 1], lane);
+        if (!do_k) continue;
+        const v16f dp = row_product<T, DP>(gt, 32 * qb, v, v16f{}, lane);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 delta = *reinterpret_cast<const float4*>(qv.delta + 32 * qb + 8 * g + 4 * half);
@@ -305,13 +318,24 @@ __global__ __launch_bounds__(ATT_NT, DP * (int)sizeof(T) <= 128 ? 2 : 1) void at
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[4 * g + r] *= dp[4 * g + r] - de[r];
         }
-        column_product<T, DP>(qt, 32 * qb, s, dk, lane);
+        column_product<T, DP>(qt, 32 * qb, s, sum[0], lane);
       }
     }
   }
   const int64_t row = ((at.b * p.nk + ki) * p.kv_heads + at.h) * p.dim;
-  store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, dk, p.scale, p.dim, a.whole, half);
-  store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, dv, 1.0f, p.dim, a.whole, half);
+  if (do_k) store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, sum[0], p.scale, p.dim, a.whole, half);
+  if (do_v) store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, sum[SPLIT ? 0 : 1], 1.0f, p.dim, a.whole, half);
+}
+
+// Bytes of a workgroup's bucket sums in the first launch.
+size_t sums_lds(const fx_attention& p, int waves) {
+  return waves * (128 + (p.dtype == FX_F32 ? 256 : 384) * (size_t)p.buckets);
+}
+
+// Waves of a workgroup of the first launch: eight where the rows are long (they leave the registers for two waves a
+// SIMD only if the tile's loads are shared by eight) and the bucket sums of eight fit, else four.
+int dq_waves(const fx_attention& p) {
+  return p.dim > 64 && p.dtype != FX_F32 && p.nq > 128 && p.buckets <= 32 && p.radius <= 1024 ? 8 : 4;
 }
 
 int64_t delta_floats(const fx_attention& p) { return cdiv(p.batch * p.heads * p.nq, 4) * 4; }
@@ -327,7 +351,7 @@ extern "C" {
 
 size_t fx_attention_grad_workspace(const fx_attention* p) {
   if (!attention_sizes_ok(p) || p->batch == 0 || p->nq == 0) return 0;
-  const int64_t tiles = cdiv(p->nq, 32 * ATT_WAVES);
+  const int64_t tiles = cdiv(p->nq, 32 * dq_waves(*p));
   return sizeof(float) * (size_t)(delta_floats(*p) + (p->table ? p->batch * p->heads * tiles * p->buckets : 0));
 }
 
@@ -356,7 +380,7 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
   }
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + delta_floats(*p);
-  const int qtiles = (int)cdiv(p->nq, 32 * ATT_WAVES), ktiles = (int)cdiv(p->nk, 32 * ATT_WAVES);
+  const int waves = dq_waves(*p), qtiles = (int)cdiv(p->nq, 32 * waves), ktiles = (int)cdiv(p->nk, 128);
   if (p->batch * p->heads * qtiles > 0x7fffffff || p->batch * p->kv_heads * ktiles > 0x7fffffff)
     return FX_ERR_UNSUPPORTED;
   const int st = attention_shape(*p, [&](auto t, auto dp, auto gen) {
@@ -364,18 +388,31 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
     const size_t tiles = tiles_lds<T, DP>(), view = view_lds(GEN, p->radius);
-    const size_t sums = ATT_WAVES * (128 + (sizeof(T) == 2 ? 384 : 256) * (size_t)p->buckets);
-    const size_t lds_q = tiles + 272 + view + (p->grad_table ? sums : 0);
+    const size_t lds_q = tiles + 272 + view + (p->grad_table ? sums_lds(*p, waves) : 0);
     const size_t lds_kv = tiles + 1040 + view;
+    constexpr bool LONG_ROWS = DP == 128 && sizeof(T) == 2;
     if (qtiles) {
       a.tiles = qtiles;
       a.items = p->batch * p->heads * qtiles;
-      hipLaunchKernelGGL((attention_dq_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds_q, s, a);
+      auto go = [&](auto w) {
+        constexpr int WAVES = decltype(w)::value;
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP, GEN, WAVES>), dim3((unsigned)a.items), dim3(64 * WAVES), lds_q, s,
+                           a);
+      };
+      if constexpr (LONG_ROWS) {
+        if (waves == 8)
+          go(ic<8>{});
+        else
+          go(ic<4>{});
+      } else {
+        go(ic<4>{});
+      }
     }
     if (ktiles) {
       a.tiles = ktiles;
       a.items = p->batch * p->kv_heads * ktiles;
-      hipLaunchKernelGGL((attention_dkv_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds_kv, s, a);
+      hipLaunchKernelGGL((attention_dkv_kernel<T, DP, GEN, LONG_ROWS>), dim3((unsigned)a.items),
+                         dim3(LONG_ROWS ? 512 : 256), lds_kv, s, a);
     }
   });
   if (st != FX_OK || !p->grad_table) return st;

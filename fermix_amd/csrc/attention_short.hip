@@ -13,6 +13,7 @@ namespace net {
 namespace {
 
 constexpr int SHORT = 128;  // queries and keys
+constexpr int SHORT_WAVES = 4, SHORT_NT = 64 * SHORT_WAVES;
 
 template <class T, int DP>
 constexpr size_t short_tile() {
@@ -22,12 +23,12 @@ constexpr int PS = SHORT + 8;  // row of P or dS in LDS
 
 template <class T, int DP>
 constexpr size_t short_lds(size_t view, int buckets, bool table) {
-  const size_t sums = table ? ATT_WAVES * 256 * (size_t)buckets : 0, ps = (size_t)SHORT * PS * sizeof(T);
+  const size_t sums = table ? SHORT_WAVES * 256 * (size_t)buckets : 0, ps = (size_t)SHORT * PS * sizeof(T);
   return 2 * short_tile<T, DP>() + 544 + view + (sums > ps ? sums : ps);
 }
 
 template <class T, int DP, bool GEN>
-__global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad_kernel(const AttArgs a) {
+__global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_grad_kernel(const AttArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   using M = Mma<T>;
   const fx_attention& p = a.p;
@@ -43,7 +44,7 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   float* const ds_sums = reinterpret_cast<float*>(rest);  // [wave][bucket][64]
   T* const ps = reinterpret_cast<T*>(rest);               // then [query][key]
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.heads, 1);
+  const Place at(xcd_item(blockIdx.x, a.items), p.heads, 1, true);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int qi = 32 * wave + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   {
     const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + at.h * p.kh;
     const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + at.h * p.vh;
-    TileLoad<T, DP> kl[2], vl[2];
+    TileLoad<T, DP, SHORT_NT> kl[2], vl[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int k0 = i * ATT_TILE;
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
     }
     q.load(static_cast<const T*>(p.q) + at.b * p.qb + (int64_t)qi * p.qn + at.h * p.qh, in, p.dim, a.whole, half);
     g.load(static_cast<const T*>(p.grad_out) + row * p.dim, in, p.dim, a.whole, half);
-    load_bias<GEN>(p, at.h, bv, a.inv_scale);
+    load_bias<GEN, SHORT_NT>(p, at.h, bv, a.inv_scale);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       kl[i].put(t0 + i * ATT_TILE * ST);
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   const bool exact = __any(fabsf(ml.x * a.c) > BASE_MAX);
   __syncthreads();
   if (!GEN) {
-    lay_bias<GEN>(bv);
+    lay_bias<GEN, SHORT_NT>(bv);
     __syncthreads();
   }
 
@@ -151,13 +152,13 @@ __global__ __launch_bounds__(ATT_NT, DP <= 64 ? 2 : 1) void attention_short_grad
   if (p.grad_table) {
     float* out = a.part + (at.h * p.batch + at.b) * p.buckets;
     // four lanes a bucket, one for each wave's sums
-    for (int t = threadIdx.x / ATT_WAVES; t < p.buckets; t += ATT_NT / ATT_WAVES) {
-      const float* w = ds_sums + ((threadIdx.x % ATT_WAVES) * p.buckets + t) * 64;
+    for (int t = threadIdx.x / SHORT_WAVES; t < p.buckets; t += SHORT_NT / SHORT_WAVES) {
+      const float* w = ds_sums + ((threadIdx.x % SHORT_WAVES) * p.buckets + t) * 64;
       float x = 0.0f;
 #pragma unroll 8
       for (int l = 0; l < 64; ++l) x += w[(l + threadIdx.x) & 63];  // rotated: no shared bank
-      x = group_sum<ATT_WAVES>(x);
-      if (threadIdx.x % ATT_WAVES == 0) out[t] = x;
+      x = group_sum<SHORT_WAVES>(x);
+      if (threadIdx.x % SHORT_WAVES == 0) out[t] = x;
     }
   }
 
@@ -220,7 +221,7 @@ int launch_attention_grad_short(const AttArgs& a, hipStream_t s) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
     const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius), p.buckets, p.grad_table != nullptr);
-    hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(ATT_NT), lds, s, a);
+    hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(SHORT_NT), lds, s, a);
   };
   return attention_shape(p, [&](auto t, auto dp, auto gen) {
     if constexpr (sizeof(t) == 2) go(t, dp, gen);
