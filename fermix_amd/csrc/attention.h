@@ -17,6 +17,19 @@ namespace net {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
+// Rows of DP elements in LDS, padded by 16 bytes. For the 16-bit types the rows of each sixteen are stored
+// transposed as 4 x 4, so that a column operand's four consecutive rows lie four apart: 16 banks apart for every DP,
+// where in order they were 4 (6 clk more for each read). A row operand's lanes meet all banks either way.
+template <class T, int DP>
+struct Tile {
+  static constexpr int STRIDE = DP + 16 / (int)sizeof(T);
+  static __device__ __forceinline__ int row_at(int row) {
+    return sizeof(T) == 2 ? (row & ~15) | ((row & 3) << 2) | ((row >> 2) & 3) : row;
+  }
+  // Place of an element; the rest of its row follows.
+  static __device__ __forceinline__ int at(int row, int col) { return row_at(row) * STRIDE + col; }
+};
+
 template <class T>
 struct Mma;
 
@@ -29,9 +42,11 @@ struct Mma<float> {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ frag columns(const float* tile, int stride, int row, int col, int lane) {
-    const float* p = tile + (row + 4 * (lane >> 5)) * stride + col + (lane & 31);
-    return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
+  template <int DP>
+  static __device__ __forceinline__ frag columns(const float* tile, int row, int col, int lane) {
+    constexpr int S = Tile<float, DP>::STRIDE;
+    const float* p = tile + (row + 4 * (lane >> 5)) * S + col + (lane & 31);
+    return frag{p[0], p[S], p[2 * S], p[3 * S]};
   }
   static __device__ __forceinline__ frag from_acc(const v16f& x, int s) {
     return frag{x[4 * s], x[4 * s + 1], x[4 * s + 2], x[4 * s + 3]};
@@ -51,9 +66,12 @@ template <class T>
 struct Mma16 {
   static constexpr int KS = 16;
   using frag = vec_t<T, 8>;
-  static __device__ __forceinline__ frag columns(const T* tile, int stride, int row, int col, int lane) {
-    const T* p = tile + (row + 4 * (lane >> 5) + ((lane & 15) >> 2)) * stride + col + (lane & 16) + 4 * (lane & 3);
-    const s16x4 a = read_columns4(p), b = read_columns4(p + 8 * stride);
+  template <int DP>
+  static __device__ __forceinline__ frag columns(const T* tile, int row, int col, int lane) {
+    // rows row + 4 half + 0..3 and those 8 on, row a multiple of 16, where Tile::row_at has them
+    constexpr int S = Tile<T, DP>::STRIDE;
+    const T* const p = tile + row * S + (((lane & 12) + (lane >> 5)) * S + (lane & 16) + 4 * (lane & 3)) + col;
+    const s16x4 a = read_columns4(p), b = read_columns4(p + 2 * S);
     return __builtin_bit_cast(frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   static __device__ __forceinline__ frag from_acc(const v16f& x, int s) {
@@ -105,11 +123,6 @@ __device__ __forceinline__ void exp_block(v16f& s, float c, float m, float base,
 
 constexpr int ATT_TILE = 64;  // rows of a staged tile
 
-template <class T>
-constexpr int tile_stride(int dp) {
-  return dp + 16 / (int)sizeof(T);
-}
-
 // A tile of up to 64 rows of dim elements, through registers into LDS: fetch starts the loads, put
 // stores them. Rows at or past `rows`, and those that `live` refuses, become zero, so that nothing a
 // masked row holds enters a product; columns dim .. DP too.
@@ -141,7 +154,7 @@ struct TileLoad {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = i * NT + threadIdx.x, r = at / CHUNKS, c = (at % CHUNKS) * V;
-      *reinterpret_cast<vec_t<T, V>*>(tile + r * tile_stride<T>(DP) + c) = x[i];
+      *reinterpret_cast<vec_t<T, V>*>(tile + Tile<T, DP>::at(r, c)) = x[i];
     }
   }
 };
@@ -171,11 +184,11 @@ struct RowFrags {
   }
 };
 
-// acc += (rows row0 .. row0 + 31 of the tile) x (the wave's rows): the tile's rows are the accumulator's.
+// acc += (rows row0 .. row0 + 31 of the tile, row0 a multiple of 16) x (the wave's rows): the tile's rows are the accumulator's.
 template <class T, int DP>
 __device__ __forceinline__ v16f row_product(const T* tile, int row0, const RowFrags<T, DP>& b, v16f acc, int lane) {
   using M = Mma<T>;
-  const T* p = tile + (row0 + (lane & 31)) * tile_stride<T>(DP) + (M::KS / 2) * (lane >> 5);
+  const T* p = tile + row0 * Tile<T, DP>::STRIDE + Tile<T, DP>::at(lane & 31, (M::KS / 2) * (lane >> 5));
 #pragma unroll
   for (int s = 0; s < RowFrags<T, DP>::STEPS; ++s)
     acc = M::mma(*reinterpret_cast<const typename M::frag*>(p + M::KS * s), b.f[s], acc);
@@ -191,7 +204,7 @@ __device__ __forceinline__ void column_product(const T* tile, int row0, const v1
     const typename M::frag b = M::from_acc(p, s);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
-      acc[d] = M::mma(M::columns(tile, tile_stride<T>(DP), row0 + M::KS * s, 32 * d, lane), b, acc[d]);
+      acc[d] = M::mma(M::template columns<DP>(tile, row0 + M::KS * s, 32 * d, lane), b, acc[d]);
   }
 }
 

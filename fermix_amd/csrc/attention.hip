@@ -13,7 +13,7 @@ namespace {
 
 template <class T, int DP>
 constexpr size_t forward_lds(bool gen, int radius) {
-  return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T) + (gen ? 272 : 0) + view_lds(gen, radius);
+  return 2 * (size_t)ATT_TILE * Tile<T, DP>::STRIDE * sizeof(T) + (gen ? 272 : 0) + view_lds(gen, radius);
 }
 
 // WAVES: of a workgroup. Two waves a SIMD hide each other's waits (head dimension 128: 1411 -> 820 us at
@@ -23,7 +23,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
   constexpr int NT = 64 * WAVES;
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention& p = a.p;
-  constexpr int DB = DP / 32, TS = ATT_TILE * tile_stride<T>(DP);
+  constexpr int DB = DP / 32, TS = ATT_TILE * Tile<T, DP>::STRIDE;
   T* const kt = reinterpret_cast<T*>(smem);
   T* const vt = kt + TS;
   unsigned char* rest = reinterpret_cast<unsigned char*>(vt + TS);

@@ -21,7 +21,7 @@ namespace {
 
 template <class T, int DP>
 constexpr size_t tiles_lds() {
-  return 2 * (size_t)ATT_TILE * tile_stride<T>(DP) * sizeof(T);
+  return 2 * (size_t)ATT_TILE * Tile<T, DP>::STRIDE * sizeof(T);
 }
 // WAVES: of a workgroup.
 template <class T, int DP, bool GEN, int WAVES>
@@ -31,7 +31,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 128 || WAVES == 
   extern __shared__ __align__(16) unsigned char smem[];
   using M = Mma<T>;
   const fx_attention& p = a.p;
-  constexpr int DB = DP / 32, TS = ATT_TILE * tile_stride<T>(DP);
+  constexpr int DB = DP / 32, TS = ATT_TILE * Tile<T, DP>::STRIDE;
   T* const kt = reinterpret_cast<T*>(smem);
   T* const vt = kt + TS;
   unsigned char* rest = reinterpret_cast<unsigned char*>(vt + TS);
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, DP * (int)sizeof(T) <= 128 || SP
   constexpr int NT = SPLIT ? 512 : 256;
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention& p = a.p;
-  constexpr int DB = DP / 32, TS = ATT_TILE * tile_stride<T>(DP);
+  constexpr int DB = DP / 32, TS = ATT_TILE * Tile<T, DP>::STRIDE;
   T* const qt = reinterpret_cast<T*>(smem);
   T* const gt = qt + TS;
   unsigned char* rest = reinterpret_cast<unsigned char*>(gt + TS);

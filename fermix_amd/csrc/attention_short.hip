@@ -17,13 +17,12 @@ constexpr int SHORT_WAVES = 4, SHORT_NT = 64 * SHORT_WAVES;
 
 template <class T, int DP>
 constexpr size_t short_tile() {
-  return (size_t)SHORT * tile_stride<T>(DP) * sizeof(T);
+  return (size_t)SHORT * Tile<T, DP>::STRIDE * sizeof(T);
 }
-constexpr int PS = SHORT + 8;  // row of P or dS in LDS
 
 template <class T, int DP>
 constexpr size_t short_lds(size_t view, int buckets, bool table) {
-  const size_t sums = table ? SHORT_WAVES * 256 * (size_t)buckets : 0, ps = (size_t)SHORT * PS * sizeof(T);
+  const size_t sums = table ? SHORT_WAVES * 256 * (size_t)buckets : 0, ps = short_tile<T, SHORT>();
   return 2 * short_tile<T, DP>() + 544 + view + (sums > ps ? sums : ps);
 }
 
@@ -32,7 +31,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
   extern __shared__ __align__(16) unsigned char smem[];
   using M = Mma<T>;
   const fx_attention& p = a.p;
-  constexpr int DB = DP / 32, ST = tile_stride<T>(DP);
+  constexpr int DB = DP / 32, ST = Tile<T, DP>::STRIDE;
   T* const t0 = reinterpret_cast<T*>(smem);  // K, then the queries
   T* const t1 = t0 + SHORT * ST;             // V, then the cotangent
   unsigned char* rest = reinterpret_cast<unsigned char*>(t1 + SHORT * ST);
@@ -165,7 +164,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
   // the wave's rows of q and dO for K and V; P
 #pragma unroll
   for (int i = 0; i < RowFrags<T, DP>::STEPS; ++i) {
-    const int o = qi * ST + M::KS * i + M::KS / 2 * half;
+    const int o = Tile<T, DP>::at(qi, M::KS * i + M::KS / 2 * half);
     *reinterpret_cast<typename M::frag*>(t0 + o) = q.f[i];
     *reinterpret_cast<typename M::frag*>(t1 + o) = g.f[i];
   }
@@ -175,9 +174,10 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         // registers 8 i ..: keys 16 i + 4 half + 0..3, then those 8 on
-        T* o = ps + qi * PS + 32 * kb + 16 * i + 4 * half;
-        *reinterpret_cast<vec_t<T, 4>*>(o) = __builtin_shufflevector(x[kb][i], x[kb][i], 0, 1, 2, 3);
-        *reinterpret_cast<vec_t<T, 4>*>(o + 8) = __builtin_shufflevector(x[kb][i], x[kb][i], 4, 5, 6, 7);
+        const int c = 32 * kb + 16 * i + 4 * half;
+        using P = Tile<T, SHORT>;
+        *reinterpret_cast<vec_t<T, 4>*>(ps + P::at(qi, c)) = __builtin_shufflevector(x[kb][i], x[kb][i], 0, 1, 2, 3);
+        *reinterpret_cast<vec_t<T, 4>*>(ps + P::at(qi, c + 8)) = __builtin_shufflevector(x[kb][i], x[kb][i], 4, 5, 6, 7);
       }
   };
   // rows: the tile's columns; columns: the wave's keys; contracted over the queries
@@ -187,9 +187,9 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
 #pragma unroll
     for (int s = 0; s < SHORT / M::KS; ++s) {
       if (M::KS * s >= qlen) break;
-      const typename M::frag b = M::columns(ps, PS, M::KS * s, 32 * wave, lane);
+      const typename M::frag b = M::template columns<SHORT>(ps, M::KS * s, 32 * wave, lane);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) acc[d] = M::mma(M::columns(tile, ST, M::KS * s, 32 * d, lane), b, acc[d]);
+      for (int d = 0; d < DB; ++d) acc[d] = M::mma(M::template columns<DP>(tile, M::KS * s, 32 * d, lane), b, acc[d]);
     }
   };
   __syncthreads();  // the bucket sums have been read
