@@ -107,7 +107,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 128 || WAVES == 
     const bool edge = k0 + ATT_TILE > klen || q0 + 32 * wave + 32 > qlen ||
                       (p.causal && k0 + ATT_TILE - 1 > wave_last - 31);
     const int far = GEN ? 0 : far_side(k0 - (p.offset + q0 + 32 * wave), ATT_TILE, 32, p.radius);
-#pragma unroll
+#pragma unroll 1  // both blocks at once spill at DP = 128: 1269 us at 2 x 16 x 8192 queries, one by one 1120
     for (int kb = 0; kb < 2; ++kb) {
       v16f s = bias_block<GEN>(p, bv, kv, kb, k0, qpos, half, far);
       s = row_product<T, DP>(kt, 32 * kb, q, s, lane);

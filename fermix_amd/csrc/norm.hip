@@ -36,27 +36,26 @@ __device__ __forceinline__ int column(int t, int e) {
   return VECT ? ((e / V) * TPR + t) * V + e % V : e * TPR + t;
 }
 
+// A lane's part of a row as it is in memory, so that the next row's can be on its way while one is worked on.
 template <class T, int TPR, int EPT, bool VECT>
-__device__ __forceinline__ void load_row(const void* base, int64_t at, int t, int C, float (&x)[EPT]) {
-  const T* p = static_cast<const T*>(base) + at;
-  if constexpr (VECT) {
-    constexpr int V = VEC16<T>;
+struct Raw {
+  static constexpr int V = VECT ? VEC16<T> : 1;
+  vec_t<T, V> v[EPT / V];
+
+  __device__ __forceinline__ void load(const void* base, int64_t at, int t, int C) {
+    const T* p = static_cast<const T*>(base) + at;
 #pragma unroll
-    for (int e = 0; e < EPT; e += V) {
-      const int c = column<T, TPR, VECT>(t, e);
-      vec_t<T, V> v = {};
-      if (c < C) v = *reinterpret_cast<const vec_t<T, V>*>(p + c);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[e + i] = (float)v[i];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      const int c = column<T, TPR, VECT>(t, e);
-      x[e] = c < C ? (float)p[c] : 0.0f;
+    for (int i = 0; i < EPT / V; ++i) {
+      const int c = column<T, TPR, VECT>(t, i * V);
+      v[i] = {};
+      if (c < C) v[i] = *reinterpret_cast<const vec_t<T, V>*>(p + c);
     }
   }
-}
+  __device__ __forceinline__ void get(float (&x)[EPT]) const {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) x[e] = (float)v[e / V][e % V];
+  }
+};
 
 template <class T, int TPR, int EPT, bool VECT>
 __device__ __forceinline__ void store_row(void* base, int64_t at, int t, int C, const float (&x)[EPT]) {
@@ -93,15 +92,24 @@ __device__ __forceinline__ void load_columns(const void* base, bool wide, float 
 
 // The gate of a row: per element, or one value.
 template <class T, int TPR, int EPT, bool VECT>
-__device__ __forceinline__ void load_gate(const fx_residual_norm& p, int64_t at, int t, float (&g)[EPT]) {
-  if (p.gc) {
-    load_row<T, TPR, EPT, VECT>(p.gate, at, t, p.columns, g);
-  } else {
-    const float v = (float)static_cast<const T*>(p.gate)[at];
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) g[e] = v;
+struct RawGate : Raw<T, TPR, EPT, VECT> {
+  T one;
+  __device__ __forceinline__ void load(const fx_residual_norm& p, int64_t at, int t) {
+    if (!p.gate) return;
+    if (p.gc)
+      Raw<T, TPR, EPT, VECT>::load(p.gate, at, t, p.columns);
+    else
+      one = static_cast<const T*>(p.gate)[at];
   }
-}
+  __device__ __forceinline__ void get(const fx_residual_norm& p, float (&g)[EPT]) const {
+    if (p.gate && p.gc) {
+      Raw<T, TPR, EPT, VECT>::get(g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) g[e] = p.gate ? (float)one : 1.0f;
+    }
+  }
+};
 
 // Sum of two values over the TPR lanes of a row; with TPR > 64 through LDS (one row a workgroup,
 // every lane calls it).
@@ -168,37 +176,45 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(const NormArgs 
   for (int e = 0; e < EPT; ++e) s[e] *= p.alpha;
   const int64_t total = p.samples * p.rows, step = (int64_t)gridDim.x * GROUPS;
   const int64_t ds = step / p.rows, dr = step - ds * p.rows;
-  const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
-  int64_t sample = first / p.rows, row = first - sample * p.rows;
-  // Every group of a workgroup makes the same number of turns (the sums over several waves meet
-  // at barriers); a turn past the last row stores nothing.
-  for (int64_t at = (int64_t)blockIdx.x * GROUPS; at < total; at += step) {
-    const bool live = at + group < total;
-    const int64_t ls = live ? sample : 0, lr = live ? row : 0;
+  int64_t first = (int64_t)blockIdx.x * GROUPS;
+  int64_t sample = (first + group) / p.rows, row = first + group - sample * p.rows;
+  Raw<T, TPR, EPT, VECT> rx, rh;
+  RawGate<T, TPR, EPT, VECT> rg;
+  auto fetch = [&](int64_t s, int64_t r) {
+    rx.load(p.x, s * p.xs + r * p.xr, t, C);
+    rh.load(p.h, s * p.hs + r * p.hr, t, C);
+    rg.load(p, s * p.gs + r * p.gr, t);
+  };
+  // Every group of a workgroup makes the same number of turns (the sums over several waves meet at
+  // barriers); a turn past the last row reads the first and stores nothing.
+  bool live = first + group < total;
+  fetch(live ? sample : 0, live ? row : 0);
+  while (first < total) {
     float x[EPT], h[EPT], g[EPT];
-    load_row<T, TPR, EPT, VECT>(p.x, ls * p.xs + lr * p.xr, t, C, x);
-    load_row<T, TPR, EPT, VECT>(p.h, ls * p.hs + lr * p.hr, t, C, h);
-    if (p.gate) load_gate<T, TPR, EPT, VECT>(p, ls * p.gs + lr * p.gr, t, g);
+    rx.get(x);
+    rh.get(h);
+    rg.get(p, g);
+    const int64_t out = sample * p.os + row * p.or_, stat = sample * p.rows + row;
+    const bool stores = live;
+    first += step;
+    sample += ds;
+    row += dr;
+    if (row >= p.rows) row -= p.rows, ++sample;
+    live = first + group < total;
+    if (first < total) fetch(live ? sample : 0, live ? row : 0);
+
     float2 s1 = make_float2(0.0f, 1.0f), s2 = make_float2(0.0f, 1.0f);
     if (p.flags & FX_NORM_POST) s1 = norm_row<T, TPR, EPT, VECT>(h, t, C, inv_c, layer, p.eps, lds);
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      const float u = p.gate ? s[e] * g[e] : s[e];
-      x[e] += u * (h[e] * w1[e] + b1[e]);
-    }
-    const int64_t out = ls * p.os + lr * p.or_;
-    if (live) store_row<T, TPR, EPT, VECT>(p.y, out, t, C, x);
+    for (int e = 0; e < EPT; ++e) x[e] += s[e] * g[e] * (h[e] * w1[e] + b1[e]);
+    if (stores) store_row<T, TPR, EPT, VECT>(p.y, out, t, C, x);
     if (p.flags & FX_NORM_PRE) {
       s2 = norm_row<T, TPR, EPT, VECT>(x, t, C, inv_c, layer, p.eps, lds);
 #pragma unroll
       for (int e = 0; e < EPT; ++e) x[e] = x[e] * w2[e] + b2[e];
-      if (live) store_row<T, TPR, EPT, VECT>(p.z, out, t, C, x);
+      if (stores) store_row<T, TPR, EPT, VECT>(p.z, out, t, C, x);
     }
-    if (p.stats && live && t == 0)
-      reinterpret_cast<float4*>(p.stats)[sample * p.rows + row] = make_float4(s1.x, s1.y, s2.x, s2.y);
-    sample += ds;
-    row += dr;
-    if (row >= p.rows) row -= p.rows, ++sample;
+    if (p.stats && stores && t == 0) reinterpret_cast<float4*>(p.stats)[stat] = make_float4(s1.x, s1.y, s2.x, s2.y);
   }
 }
 
@@ -231,27 +247,41 @@ __device__ __forceinline__ void columns_out(const float (&v)[EPT], float* lds, i
   }
 }
 
-template <class T, int TPR, int EPT, bool VECT>
+// BIAS: layer norm or a bias; without, the means and the biases' sums do not take registers.
+template <class T, int TPR, int EPT, bool VECT, bool BIAS>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const NormArgs a) {
   constexpr int GROUPS = norm_threads(TPR) / TPR;
   __shared__ float2 lds[TPR > 64 ? TPR / 64 : 1];
   __shared__ float sums[GROUPS > 1 ? GROUPS * EPT * TPR : 1];
   const fx_residual_norm& p = a.p;
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, C = p.columns;
-  const bool wide = p.wdtype == FX_F32, layer = p.flags & FX_NORM_LAYER;
+  const bool wide = p.wdtype == FX_F32, layer = BIAS && (p.flags & FX_NORM_LAYER);
   const bool post = p.flags & FX_NORM_POST, pre = (p.flags & FX_NORM_PRE) && p.grad_z;
   const float inv_c = 1.0f / (float)C;
   float w1[EPT], b1[EPT], s[EPT], w2[EPT];
   load_columns<T, TPR, EPT, VECT>(p.post_weight, wide, 1.0f, t, C, w1);
-  load_columns<T, TPR, EPT, VECT>(p.post_bias, wide, 0.0f, t, C, b1);
+  load_columns<T, TPR, EPT, VECT>(BIAS ? p.post_bias : nullptr, wide, 0.0f, t, C, b1);
   load_columns<T, TPR, EPT, VECT>(p.scale, wide, 1.0f, t, C, s);
   load_columns<T, TPR, EPT, VECT>(p.pre_weight, wide, 1.0f, t, C, w2);
+#pragma unroll
+  for (int e = 0; e < EPT; ++e) s[e] *= p.alpha;
   float dw1[EPT], db1[EPT], dsc[EPT], dw2[EPT], db2[EPT];
 #pragma unroll
   for (int e = 0; e < EPT; ++e) dw1[e] = db1[e] = dsc[e] = dw2[e] = db2[e] = 0.0f;
   const bool gate_rows = p.gate && p.gr && p.gc;   // a gradient per element
   const bool gate_row = p.gate && p.gr && !p.gc;   // one per row
   const bool gate_sum = p.gate && !p.gr;           // summed over the rows of a sample
+  Raw<T, TPR, EPT, VECT> rx, rh, ry = {}, rz = {};  // zero without a cotangent
+  RawGate<T, TPR, EPT, VECT> rg;
+  float4 rs;
+  auto fetch = [&](int64_t sample, int64_t row) {
+    rx.load(p.x, sample * p.xs + row * p.xr, t, C);
+    rh.load(p.h, sample * p.hs + row * p.hr, t, C);
+    if (p.grad_y) ry.load(p.grad_y, sample * p.os + row * p.or_, t, C);
+    if (pre) rz.load(p.grad_z, sample * p.os + row * p.or_, t, C);
+    rg.load(p, sample * p.gs + row * p.gr, t);
+    rs = reinterpret_cast<const float4*>(p.stats)[sample * p.rows + row];
+  };
   for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
     const int64_t sample = item / a.chunks, row0 = (item - sample * a.chunks) * a.chunk_rows;
     const int64_t left = p.rows - row0;
@@ -259,26 +289,28 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
     float dgs[EPT];
 #pragma unroll
     for (int e = 0; e < EPT; ++e) dgs[e] = 0.0f;
+    bool live = group < rows;
+    fetch(sample, row0 + (live ? group : 0));
     for (int64_t r0 = 0; r0 < rows; r0 += GROUPS) {
-      const bool live = r0 + group < rows;
       const int64_t row = row0 + (live ? r0 + group : 0);
       const int64_t io = sample * p.os + row * p.or_;
+      const bool stores = live;
       float x[EPT], h[EPT], dy[EPT], dz[EPT], g[EPT];
-      load_row<T, TPR, EPT, VECT>(p.x, sample * p.xs + row * p.xr, t, C, x);
-      load_row<T, TPR, EPT, VECT>(p.h, sample * p.hs + row * p.hr, t, C, h);
-#pragma unroll
-      for (int e = 0; e < EPT; ++e) dy[e] = dz[e] = 0.0f, g[e] = 1.0f;
-      if (p.grad_y) load_row<T, TPR, EPT, VECT>(p.grad_y, io, t, C, dy);
-      if (pre) load_row<T, TPR, EPT, VECT>(p.grad_z, io, t, C, dz);
-      if (p.gate) load_gate<T, TPR, EPT, VECT>(p, sample * p.gs + row * p.gr, t, g);
-      const float4 st = reinterpret_cast<const float4*>(p.stats)[sample * p.rows + row];
+      rx.get(x);
+      rh.get(h);
+      ry.get(dy);
+      rz.get(dz);
+      rg.get(p, g);
+      const float4 st = rs;
+      live = r0 + GROUPS + group < rows;
+      if (r0 + GROUPS < rows) fetch(sample, row0 + (live ? r0 + GROUPS + group : 0));
       // n1 in h, a in x's place of y = x + u a, n2 in x
       float av[EPT];
 #pragma unroll
       for (int e = 0; e < EPT; ++e) {
         if (post) h[e] = column<T, TPR, VECT>(t, e) < C ? (h[e] - st.x) * st.y : 0.0f;
         av[e] = h[e] * w1[e] + b1[e];
-        x[e] += p.alpha * s[e] * g[e] * av[e];
+        x[e] += s[e] * g[e] * av[e];
       }
       float2 m = make_float2(0.0f, 0.0f);
       if (pre) {
@@ -294,26 +326,26 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
         m.y = layer ? m.y * inv_c : 0.0f;
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
-          dw2[e] += live ? dz[e] * x[e] : 0.0f;
-          db2[e] += live ? dz[e] : 0.0f;
+          dw2[e] += stores ? dz[e] * x[e] : 0.0f;
+          if (BIAS) db2[e] += stores ? dz[e] : 0.0f;
           dy[e] += st.w * (dz[e] * w2[e] - x[e] * m.x - m.y);
         }
       }
-      if (live && p.grad_x) store_row<T, TPR, EPT, VECT>(p.grad_x, io, t, C, dy);
+      if (stores && p.grad_x) store_row<T, TPR, EPT, VECT>(p.grad_x, io, t, C, dy);
       float dg = 0.0f;
       m = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int e = 0; e < EPT; ++e) {
         const bool in = column<T, TPR, VECT>(t, e) < C;
-        const float d = in ? dy[e] * p.alpha : 0.0f;
+        const float d = in ? dy[e] : 0.0f;
         const float du = d * av[e];
         const float dge = du * s[e];
         dg += dge;
         const float da = d * s[e] * g[e];
-        if (live) {
+        if (stores) {
           dsc[e] += du * g[e];
           dgs[e] += dge;
-          db1[e] += da;
+          if (BIAS) db1[e] += da;
           dw1[e] += da * h[e];
         }
         x[e] = da * w1[e];  // dn1
@@ -321,7 +353,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
         m.y += x[e];
         dz[e] = dge;
       }
-      if (gate_rows && live) store_row<T, TPR, EPT, VECT>(p.grad_gate, (sample * p.rows + row) * C, t, C, dz);
+      if (gate_rows && stores) store_row<T, TPR, EPT, VECT>(p.grad_gate, (sample * p.rows + row) * C, t, C, dz);
       if (post) {
         m = row_sum<TPR>(m, lds);
         m.x *= inv_c;
@@ -329,14 +361,16 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
 #pragma unroll
         for (int e = 0; e < EPT; ++e) x[e] = st.y * (x[e] - h[e] * m.x - m.y);
       }
-      if (live && p.grad_h) store_row<T, TPR, EPT, VECT>(p.grad_h, io, t, C, x);
+      if (stores && p.grad_h) store_row<T, TPR, EPT, VECT>(p.grad_h, io, t, C, x);
       if (gate_row) {
         dg = row_sum<TPR>(make_float2(dg, 0.0f), lds).x;
-        if (live && t == 0) static_cast<T*>(p.grad_gate)[sample * p.rows + row] = (T)dg;
+        if (stores && t == 0) static_cast<T*>(p.grad_gate)[sample * p.rows + row] = (T)dg;
       }
     }
     if (gate_sum) columns_out<T, TPR, EPT, VECT>(dgs, sums, t, group, C, a.gate_part + item * C);
   }
+#pragma unroll
+  for (int e = 0; e < EPT; ++e) dsc[e] *= p.alpha;
   const int64_t plane = (int64_t)gridDim.x * C;
   float* out = a.part + blockIdx.x * (int64_t)C;
   if (p.grad_post_weight) columns_out<T, TPR, EPT, VECT>(dw1, sums, t, group, C, out + Q_W1 * plane);
@@ -346,7 +380,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
   if (p.grad_pre_bias) columns_out<T, TPR, EPT, VECT>(db2, sums, t, group, C, out + Q_B2 * plane);
 }
 
-// The workgroups' column sums added: 64 columns a workgroup, its four waves every fourth part.
+// The workgroups' column sums added: 16 columns a workgroup, its 64 rows of lanes every 64th part.
+constexpr int JOIN_COLUMNS = 16, JOIN_ROWS = 64, JOIN_NT = JOIN_COLUMNS * JOIN_ROWS;
 struct JoinArgs {
   const float* part;
   int64_t parts;
@@ -355,19 +390,25 @@ struct JoinArgs {
   void* out[Q_COLUMNS];
 };
 template <class T>
-__global__ __launch_bounds__(256) void columns_join_kernel(const JoinArgs a) {
-  __shared__ double s[4][64];
+__global__ __launch_bounds__(JOIN_NT) void columns_join_kernel(const JoinArgs a) {
+  __shared__ double s[JOIN_NT];
   void* const out = a.out[blockIdx.y];
   if (!out) return;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + l;
+  const int l = threadIdx.x % JOIN_COLUMNS, r = threadIdx.x / JOIN_COLUMNS, c = blockIdx.x * JOIN_COLUMNS + l;
   const float* p = a.part + (int64_t)blockIdx.y * a.parts * a.columns;
   double x = 0.0;
-  if (c < a.columns)
-    for (int64_t i = w; i < a.parts; i += 4) x += (double)p[i * a.columns + c];
-  s[w][l] = x;
+  if (c < a.columns) {
+#pragma unroll 8
+    for (int64_t i = r; i < a.parts; i += JOIN_ROWS) x += (double)p[i * a.columns + c];
+  }
+  s[threadIdx.x] = x;
   __syncthreads();
-  if (w == 0 && c < a.columns) {
-    x = s[0][l] + s[1][l] + s[2][l] + s[3][l];
+  for (int m = JOIN_ROWS / 2; m; m >>= 1) {
+    if (r < m) s[threadIdx.x] += s[threadIdx.x + m * JOIN_COLUMNS];
+    __syncthreads();
+  }
+  if (r == 0 && c < a.columns) {
+    x = s[l];
     if (a.wide)
       static_cast<float*>(out)[c] = (float)x;
     else
@@ -535,15 +576,20 @@ int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t wor
     using T = decltype(t);
     if (!none) {
       norm_shape(p->columns, norm_vectors(*p), [&](auto tpr, auto ept, auto vect) {
-        constexpr int TPR = decltype(tpr)::value;
-        hipLaunchKernelGGL((norm_grad_kernel<T, TPR, decltype(ept)::value, decltype(vect)::value != 0>),
-                           dim3((unsigned)n.groups), dim3(norm_threads(TPR)), 0, s, a);
+        constexpr int TPR = decltype(tpr)::value, EPT = decltype(ept)::value;
+        constexpr bool VECT = decltype(vect)::value != 0;
+        const dim3 grid((unsigned)n.groups), block(norm_threads(TPR));
+        if ((p->flags & FX_NORM_LAYER) || p->post_bias || p->pre_bias)
+          hipLaunchKernelGGL((norm_grad_kernel<T, TPR, EPT, VECT, true>), grid, block, 0, s, a);
+        else
+          hipLaunchKernelGGL((norm_grad_kernel<T, TPR, EPT, VECT, false>), grid, block, 0, s, a);
       });
       if (launched() != FX_OK) return FX_ERR_LAUNCH;
     }
     JoinArgs j{a.part, n.groups, p->columns, p->wdtype == FX_F32,
                {p->grad_post_weight, p->grad_post_bias, p->grad_scale, p->grad_pre_weight, p->grad_pre_bias}};
-    hipLaunchKernelGGL((columns_join_kernel<T>), dim3((p->columns + 63) / 64, Q_COLUMNS), dim3(256), 0, s, j);
+    hipLaunchKernelGGL((columns_join_kernel<T>), dim3((p->columns + JOIN_COLUMNS - 1) / JOIN_COLUMNS, Q_COLUMNS),
+                       dim3(JOIN_NT), 0, s, j);
     if (!none && p->gate && !p->gr)
       hipLaunchKernelGGL((gate_join_kernel<T>), dim3((unsigned)p->samples, p->gc ? (p->columns + 255) / 256 : 1),
                          dim3(256), 0, s, a.gate_part, p->samples, n.chunks, p->columns, (int)p->gc,
