@@ -26,29 +26,40 @@ struct NormArgs {
   float* gate_part;   // items' gate sums [item][columns]
 };
 
+constexpr int EPT = 8;  // elements of a lane
+
 enum { Q_W1, Q_B1, Q_S, Q_W2, Q_B2, Q_COLUMNS };
 
-// Column of element e of lane t: vectors of 16 bytes, or single elements where the rows are not
-// 16-byte aligned.
-template <class T, int TPR, bool VECT>
+// Column of element e of lane t: vectors of V elements, a row's lanes side by side.
+template <int V, int TPR>
 __device__ __forceinline__ int column(int t, int e) {
-  constexpr int V = VEC16<T>;
-  return VECT ? ((e / V) * TPR + t) * V + e % V : e * TPR + t;
+  return ((e / V) * TPR + t) * V + e % V;
 }
 
+// V: a vector of 16 bytes, aligned to its elements only (rows of odd widths); one access all the same. For float32 rows
+// that are not 16-byte aligned single elements (V = 1) are faster, 2000 x 90 rows of 333: 418 us for 481; for
+// 16-bit ones they would be two bytes each.
+template <class T, int V>
+using loose_t = T __attribute__((ext_vector_type(V), aligned(alignof(T))));
+
 // A lane's part of a row as it is in memory, so that the next row's can be on its way while one is worked on.
-template <class T, int TPR, int EPT, bool VECT>
+template <class T, int V, int TPR>
 struct Raw {
-  static constexpr int V = VECT ? VEC16<T> : 1;
   vec_t<T, V> v[EPT / V];
 
-  __device__ __forceinline__ void load(const void* base, int64_t at, int t, int C) {
+  __device__ __forceinline__ void load(const void* base, int64_t at, int t, int C, bool live) {
     const T* p = static_cast<const T*>(base) + at;
 #pragma unroll
     for (int i = 0; i < EPT / V; ++i) {
-      const int c = column<T, TPR, VECT>(t, i * V);
+      const int c = column<V, TPR>(t, i * V);
       v[i] = {};
-      if (c < C) v[i] = *reinterpret_cast<const vec_t<T, V>*>(p + c);
+      if (live && c + V <= C) {
+        v[i] = *reinterpret_cast<const loose_t<T, V>*>(p + c);
+      } else if (live && c < C) {
+#pragma unroll
+        for (int e = 0; e < V - 1; ++e)
+          if (c + e < C) v[i][e] = p[c + e];
+      }
     }
   }
   __device__ __forceinline__ void get(float (&x)[EPT]) const {
@@ -57,53 +68,50 @@ struct Raw {
   }
 };
 
-template <class T, int TPR, int EPT, bool VECT>
+template <class T, int V, int TPR>
 __device__ __forceinline__ void store_row(void* base, int64_t at, int t, int C, const float (&x)[EPT]) {
   T* p = static_cast<T*>(base) + at;
-  if constexpr (VECT) {
-    constexpr int V = VEC16<T>;
 #pragma unroll
-    for (int e = 0; e < EPT; e += V) {
-      const int c = column<T, TPR, VECT>(t, e);
-      vec_t<T, V> v;
+  for (int e = 0; e < EPT; e += V) {
+    const int c = column<V, TPR>(t, e);
+    vec_t<T, V> v;
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (T)x[e + i];
-      if (c < C) *reinterpret_cast<vec_t<T, V>*>(p + c) = v;
-    }
-  } else {
+    for (int i = 0; i < V; ++i) v[i] = (T)x[e + i];
+    if (c + V <= C) {
+      *reinterpret_cast<loose_t<T, V>*>(p + c) = v;
+    } else if (c < C) {
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) {
-      const int c = column<T, TPR, VECT>(t, e);
-      if (c < C) p[c] = (T)x[e];
+      for (int i = 0; i < V - 1; ++i)
+        if (c + i < C) p[c + i] = v[i];
     }
   }
 }
 
 // A column vector of wdtype (float32, or T), `none` where it is not given.
-template <class T, int TPR, int EPT, bool VECT>
+template <class T, int V, int TPR>
 __device__ __forceinline__ void load_columns(const void* base, bool wide, float none, int t, int C, float (&x)[EPT]) {
 #pragma unroll
   for (int e = 0; e < EPT; ++e) {
-    const int c = column<T, TPR, VECT>(t, e);
+    const int c = column<V, TPR>(t, e);
     x[e] = none;
     if (base && c < C) x[e] = wide ? static_cast<const float*>(base)[c] : (float)static_cast<const T*>(base)[c];
   }
 }
 
 // The gate of a row: per element, or one value.
-template <class T, int TPR, int EPT, bool VECT>
-struct RawGate : Raw<T, TPR, EPT, VECT> {
+template <class T, int V, int TPR>
+struct RawGate : Raw<T, V, TPR> {
   T one;
-  __device__ __forceinline__ void load(const fx_residual_norm& p, int64_t at, int t) {
+  __device__ __forceinline__ void load(const fx_residual_norm& p, int64_t at, int t, bool live) {
     if (!p.gate) return;
     if (p.gc)
-      Raw<T, TPR, EPT, VECT>::load(p.gate, at, t, p.columns);
+      Raw<T, V, TPR>::load(p.gate, at, t, p.columns, live);
     else
-      one = static_cast<const T*>(p.gate)[at];
+      one = live ? static_cast<const T*>(p.gate)[at] : T(0);
   }
   __device__ __forceinline__ void get(const fx_residual_norm& p, float (&g)[EPT]) const {
     if (p.gate && p.gc) {
-      Raw<T, TPR, EPT, VECT>::get(g);
+      Raw<T, V, TPR>::get(g);
     } else {
 #pragma unroll
       for (int e = 0; e < EPT; ++e) g[e] = p.gate ? (float)one : 1.0f;
@@ -134,7 +142,7 @@ __device__ __forceinline__ float2 row_sum(float2 v, float2* lds) {
 
 // x becomes the normed row; mean and reciprocal deviation are returned. The deviation is summed from
 // the centred row, so a large mean costs no digits. Columns past C are left 0.
-template <class T, int TPR, int EPT, bool VECT>
+template <class T, int V, int TPR>
 __device__ __forceinline__ float2 norm_row(float (&x)[EPT], int t, int C, float inv_c, bool layer, float eps,
                                            float2* lds) {
   float mean = 0.0f;
@@ -144,7 +152,7 @@ __device__ __forceinline__ float2 norm_row(float (&x)[EPT], int t, int C, float 
     for (int e = 0; e < EPT; ++e) s += x[e];
     mean = row_sum<TPR>(make_float2(s, 0.0f), lds).x * inv_c;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) x[e] = column<T, TPR, VECT>(t, e) < C ? x[e] - mean : 0.0f;
+    for (int e = 0; e < EPT; ++e) x[e] = column<V, TPR>(t, e) < C ? x[e] - mean : 0.0f;
   }
   float s = 0.0f;
 #pragma unroll
@@ -158,7 +166,7 @@ __device__ __forceinline__ float2 norm_row(float (&x)[EPT], int t, int C, float 
 // One row a workgroup where it takes several waves, else 256 lanes of row groups.
 constexpr int norm_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }
 
-template <class T, int TPR, int EPT, bool VECT>
+template <class T, int V, int TPR>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(const NormArgs a) {
   constexpr int GROUPS = norm_threads(TPR) / TPR;
   __shared__ float2 lds[TPR > 64 ? TPR / 64 : 1];
@@ -167,28 +175,28 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(const NormArgs 
   const bool wide = p.wdtype == FX_F32, layer = p.flags & FX_NORM_LAYER;
   const float inv_c = 1.0f / (float)C;
   float w1[EPT], b1[EPT], s[EPT], w2[EPT], b2[EPT];
-  load_columns<T, TPR, EPT, VECT>(p.post_weight, wide, 1.0f, t, C, w1);
-  load_columns<T, TPR, EPT, VECT>(p.post_bias, wide, 0.0f, t, C, b1);
-  load_columns<T, TPR, EPT, VECT>(p.scale, wide, 1.0f, t, C, s);
-  load_columns<T, TPR, EPT, VECT>(p.pre_weight, wide, 1.0f, t, C, w2);
-  load_columns<T, TPR, EPT, VECT>(p.pre_bias, wide, 0.0f, t, C, b2);
+  load_columns<T, V, TPR>(p.post_weight, wide, 1.0f, t, C, w1);
+  load_columns<T, V, TPR>(p.post_bias, wide, 0.0f, t, C, b1);
+  load_columns<T, V, TPR>(p.scale, wide, 1.0f, t, C, s);
+  load_columns<T, V, TPR>(p.pre_weight, wide, 1.0f, t, C, w2);
+  load_columns<T, V, TPR>(p.pre_bias, wide, 0.0f, t, C, b2);
 #pragma unroll
   for (int e = 0; e < EPT; ++e) s[e] *= p.alpha;
   const int64_t total = p.samples * p.rows, step = (int64_t)gridDim.x * GROUPS;
   const int64_t ds = step / p.rows, dr = step - ds * p.rows;
   int64_t first = (int64_t)blockIdx.x * GROUPS;
   int64_t sample = (first + group) / p.rows, row = first + group - sample * p.rows;
-  Raw<T, TPR, EPT, VECT> rx, rh;
-  RawGate<T, TPR, EPT, VECT> rg;
-  auto fetch = [&](int64_t s, int64_t r) {
-    rx.load(p.x, s * p.xs + r * p.xr, t, C);
-    rh.load(p.h, s * p.hs + r * p.hr, t, C);
-    rg.load(p, s * p.gs + r * p.gr, t);
+  Raw<T, V, TPR> rx, rh;
+  RawGate<T, V, TPR> rg;
+  auto fetch = [&](int64_t s, int64_t r, bool live) {
+    rx.load(p.x, s * p.xs + r * p.xr, t, C, live);
+    rh.load(p.h, s * p.hs + r * p.hr, t, C, live);
+    rg.load(p, s * p.gs + r * p.gr, t, live);
   };
   // Every group of a workgroup makes the same number of turns (the sums over several waves meet at
-  // barriers); a turn past the last row reads the first and stores nothing.
+  // barriers); a turn past the last row works on zeros and stores nothing.
   bool live = first + group < total;
-  fetch(live ? sample : 0, live ? row : 0);
+  fetch(sample, row, live);
   while (first < total) {
     float x[EPT], h[EPT], g[EPT];
     rx.get(x);
@@ -201,31 +209,31 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_kernel(const NormArgs 
     row += dr;
     if (row >= p.rows) row -= p.rows, ++sample;
     live = first + group < total;
-    if (first < total) fetch(live ? sample : 0, live ? row : 0);
+    if (first < total) fetch(sample, row, live);
 
     float2 s1 = make_float2(0.0f, 1.0f), s2 = make_float2(0.0f, 1.0f);
-    if (p.flags & FX_NORM_POST) s1 = norm_row<T, TPR, EPT, VECT>(h, t, C, inv_c, layer, p.eps, lds);
+    if (p.flags & FX_NORM_POST) s1 = norm_row<T, V, TPR>(h, t, C, inv_c, layer, p.eps, lds);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) x[e] += s[e] * g[e] * (h[e] * w1[e] + b1[e]);
-    if (stores) store_row<T, TPR, EPT, VECT>(p.y, out, t, C, x);
+    if (stores) store_row<T, V, TPR>(p.y, out, t, C, x);
     if (p.flags & FX_NORM_PRE) {
-      s2 = norm_row<T, TPR, EPT, VECT>(x, t, C, inv_c, layer, p.eps, lds);
+      s2 = norm_row<T, V, TPR>(x, t, C, inv_c, layer, p.eps, lds);
 #pragma unroll
       for (int e = 0; e < EPT; ++e) x[e] = x[e] * w2[e] + b2[e];
-      if (stores) store_row<T, TPR, EPT, VECT>(p.z, out, t, C, x);
+      if (stores) store_row<T, V, TPR>(p.z, out, t, C, x);
     }
     if (p.stats && stores && t == 0) reinterpret_cast<float4*>(p.stats)[stat] = make_float4(s1.x, s1.y, s2.x, s2.y);
   }
 }
 
 // Sums of v over the workgroup's row groups, per column, into out[column].
-template <class T, int TPR, int EPT, bool VECT>
+template <class T, int V, int TPR>
 __device__ __forceinline__ void columns_out(const float (&v)[EPT], float* lds, int t, int group, int C, float* out) {
   constexpr int GROUPS = norm_threads(TPR) / TPR;
   if constexpr (GROUPS == 1) {
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
-      const int c = column<T, TPR, VECT>(t, e);
+      const int c = column<V, TPR>(t, e);
       if (c < C) out[c] = v[e];
     }
   } else {
@@ -240,7 +248,7 @@ __device__ __forceinline__ void columns_out(const float (&v)[EPT], float* lds, i
       if (e < EPT) {
         float sum = 0.0f;
         for (int k = 0; k < GROUPS; ++k) sum += lds[(k * EPT + e) * TPR + t];
-        const int c = column<T, TPR, VECT>(t, e);
+        const int c = column<V, TPR>(t, e);
         if (c < C) out[c] = sum;
       }
     }
@@ -248,7 +256,7 @@ __device__ __forceinline__ void columns_out(const float (&v)[EPT], float* lds, i
 }
 
 // BIAS: layer norm or a bias; without, the means and the biases' sums do not take registers.
-template <class T, int TPR, int EPT, bool VECT, bool BIAS>
+template <class T, int V, int TPR, bool BIAS>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const NormArgs a) {
   constexpr int GROUPS = norm_threads(TPR) / TPR;
   __shared__ float2 lds[TPR > 64 ? TPR / 64 : 1];
@@ -259,10 +267,10 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
   const bool post = p.flags & FX_NORM_POST, pre = (p.flags & FX_NORM_PRE) && p.grad_z;
   const float inv_c = 1.0f / (float)C;
   float w1[EPT], b1[EPT], s[EPT], w2[EPT];
-  load_columns<T, TPR, EPT, VECT>(p.post_weight, wide, 1.0f, t, C, w1);
-  load_columns<T, TPR, EPT, VECT>(BIAS ? p.post_bias : nullptr, wide, 0.0f, t, C, b1);
-  load_columns<T, TPR, EPT, VECT>(p.scale, wide, 1.0f, t, C, s);
-  load_columns<T, TPR, EPT, VECT>(p.pre_weight, wide, 1.0f, t, C, w2);
+  load_columns<T, V, TPR>(p.post_weight, wide, 1.0f, t, C, w1);
+  load_columns<T, V, TPR>(BIAS ? p.post_bias : nullptr, wide, 0.0f, t, C, b1);
+  load_columns<T, V, TPR>(p.scale, wide, 1.0f, t, C, s);
+  load_columns<T, V, TPR>(p.pre_weight, wide, 1.0f, t, C, w2);
 #pragma unroll
   for (int e = 0; e < EPT; ++e) s[e] *= p.alpha;
   float dw1[EPT], db1[EPT], dsc[EPT], dw2[EPT], db2[EPT];
@@ -271,16 +279,17 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
   const bool gate_rows = p.gate && p.gr && p.gc;   // a gradient per element
   const bool gate_row = p.gate && p.gr && !p.gc;   // one per row
   const bool gate_sum = p.gate && !p.gr;           // summed over the rows of a sample
-  Raw<T, TPR, EPT, VECT> rx, rh, ry = {}, rz = {};  // zero without a cotangent
-  RawGate<T, TPR, EPT, VECT> rg;
+  Raw<T, V, TPR> rx, rh, ry = {}, rz = {};  // zero without a cotangent
+  RawGate<T, V, TPR> rg;
   float4 rs;
-  auto fetch = [&](int64_t sample, int64_t row) {
-    rx.load(p.x, sample * p.xs + row * p.xr, t, C);
-    rh.load(p.h, sample * p.hs + row * p.hr, t, C);
-    if (p.grad_y) ry.load(p.grad_y, sample * p.os + row * p.or_, t, C);
-    if (pre) rz.load(p.grad_z, sample * p.os + row * p.or_, t, C);
-    rg.load(p, sample * p.gs + row * p.gr, t);
-    rs = reinterpret_cast<const float4*>(p.stats)[sample * p.rows + row];
+  // a row that is not live is zeros, and adds nothing to any sum
+  auto fetch = [&](int64_t sample, int64_t row, bool live) {
+    rx.load(p.x, sample * p.xs + row * p.xr, t, C, live);
+    rh.load(p.h, sample * p.hs + row * p.hr, t, C, live);
+    if (p.grad_y) ry.load(p.grad_y, sample * p.os + row * p.or_, t, C, live);
+    if (pre) rz.load(p.grad_z, sample * p.os + row * p.or_, t, C, live);
+    rg.load(p, sample * p.gs + row * p.gr, t, live);
+    rs = live ? reinterpret_cast<const float4*>(p.stats)[sample * p.rows + row] : make_float4(0.0f, 1.0f, 0.0f, 1.0f);
   };
   for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
     const int64_t sample = item / a.chunks, row0 = (item - sample * a.chunks) * a.chunk_rows;
@@ -290,9 +299,9 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
 #pragma unroll
     for (int e = 0; e < EPT; ++e) dgs[e] = 0.0f;
     bool live = group < rows;
-    fetch(sample, row0 + (live ? group : 0));
+    fetch(sample, row0 + group, live);
     for (int64_t r0 = 0; r0 < rows; r0 += GROUPS) {
-      const int64_t row = row0 + (live ? r0 + group : 0);
+      const int64_t row = row0 + r0 + group;
       const int64_t io = sample * p.os + row * p.or_;
       const bool stores = live;
       float x[EPT], h[EPT], dy[EPT], dz[EPT], g[EPT];
@@ -303,12 +312,13 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
       rg.get(p, g);
       const float4 st = rs;
       live = r0 + GROUPS + group < rows;
-      if (r0 + GROUPS < rows) fetch(sample, row0 + (live ? r0 + GROUPS + group : 0));
+      if (r0 + GROUPS < rows) fetch(sample, row + GROUPS, live);
       // n1 in h, a in x's place of y = x + u a, n2 in x
       float av[EPT];
 #pragma unroll
       for (int e = 0; e < EPT; ++e) {
-        if (post) h[e] = column<T, TPR, VECT>(t, e) < C ? (h[e] - st.x) * st.y : 0.0f;
+        // past C all is zero, but for what a mean makes of it
+        if (post) h[e] = !layer ? h[e] * st.y : column<V, TPR>(t, e) < C ? (h[e] - st.x) * st.y : 0.0f;
         av[e] = h[e] * w1[e] + b1[e];
         x[e] += s[e] * g[e] * av[e];
       }
@@ -316,7 +326,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
       if (pre) {
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
-          x[e] = column<T, TPR, VECT>(t, e) < C ? (x[e] - st.z) * st.w : 0.0f;
+          x[e] = !layer ? x[e] * st.w : column<V, TPR>(t, e) < C ? (x[e] - st.z) * st.w : 0.0f;
           const float dn = dz[e] * w2[e];
           m.x += dn * x[e];
           m.y += dn;
@@ -326,34 +336,31 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
         m.y = layer ? m.y * inv_c : 0.0f;
 #pragma unroll
         for (int e = 0; e < EPT; ++e) {
-          dw2[e] += stores ? dz[e] * x[e] : 0.0f;
-          if (BIAS) db2[e] += stores ? dz[e] : 0.0f;
+          dw2[e] += dz[e] * x[e];
+          if (BIAS) db2[e] += dz[e];
           dy[e] += st.w * (dz[e] * w2[e] - x[e] * m.x - m.y);
         }
       }
-      if (stores && p.grad_x) store_row<T, TPR, EPT, VECT>(p.grad_x, io, t, C, dy);
+      if (stores && p.grad_x) store_row<T, V, TPR>(p.grad_x, io, t, C, dy);
       float dg = 0.0f;
       m = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int e = 0; e < EPT; ++e) {
-        const bool in = column<T, TPR, VECT>(t, e) < C;
-        const float d = in ? dy[e] : 0.0f;
+        const float d = layer && column<V, TPR>(t, e) >= C ? 0.0f : dy[e];
         const float du = d * av[e];
         const float dge = du * s[e];
         dg += dge;
         const float da = d * s[e] * g[e];
-        if (stores) {
-          dsc[e] += du * g[e];
-          dgs[e] += dge;
-          if (BIAS) db1[e] += da;
-          dw1[e] += da * h[e];
-        }
+        dsc[e] += du * g[e];
+        dgs[e] += dge;
+        if (BIAS) db1[e] += da;
+        dw1[e] += da * h[e];
         x[e] = da * w1[e];  // dn1
         m.x += x[e] * h[e];
         m.y += x[e];
         dz[e] = dge;
       }
-      if (gate_rows && stores) store_row<T, TPR, EPT, VECT>(p.grad_gate, (sample * p.rows + row) * C, t, C, dz);
+      if (gate_rows && stores) store_row<T, V, TPR>(p.grad_gate, (sample * p.rows + row) * C, t, C, dz);
       if (post) {
         m = row_sum<TPR>(m, lds);
         m.x *= inv_c;
@@ -361,23 +368,23 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_grad_kernel(const Norm
 #pragma unroll
         for (int e = 0; e < EPT; ++e) x[e] = st.y * (x[e] - h[e] * m.x - m.y);
       }
-      if (stores && p.grad_h) store_row<T, TPR, EPT, VECT>(p.grad_h, io, t, C, x);
+      if (stores && p.grad_h) store_row<T, V, TPR>(p.grad_h, io, t, C, x);
       if (gate_row) {
         dg = row_sum<TPR>(make_float2(dg, 0.0f), lds).x;
         if (stores && t == 0) static_cast<T*>(p.grad_gate)[sample * p.rows + row] = (T)dg;
       }
     }
-    if (gate_sum) columns_out<T, TPR, EPT, VECT>(dgs, sums, t, group, C, a.gate_part + item * C);
+    if (gate_sum) columns_out<T, V, TPR>(dgs, sums, t, group, C, a.gate_part + item * C);
   }
 #pragma unroll
   for (int e = 0; e < EPT; ++e) dsc[e] *= p.alpha;
   const int64_t plane = (int64_t)gridDim.x * C;
   float* out = a.part + blockIdx.x * (int64_t)C;
-  if (p.grad_post_weight) columns_out<T, TPR, EPT, VECT>(dw1, sums, t, group, C, out + Q_W1 * plane);
-  if (p.grad_post_bias) columns_out<T, TPR, EPT, VECT>(db1, sums, t, group, C, out + Q_B1 * plane);
-  if (p.grad_scale) columns_out<T, TPR, EPT, VECT>(dsc, sums, t, group, C, out + Q_S * plane);
-  if (p.grad_pre_weight) columns_out<T, TPR, EPT, VECT>(dw2, sums, t, group, C, out + Q_W2 * plane);
-  if (p.grad_pre_bias) columns_out<T, TPR, EPT, VECT>(db2, sums, t, group, C, out + Q_B2 * plane);
+  if (p.grad_post_weight) columns_out<T, V, TPR>(dw1, sums, t, group, C, out + Q_W1 * plane);
+  if (p.grad_post_bias) columns_out<T, V, TPR>(db1, sums, t, group, C, out + Q_B1 * plane);
+  if (p.grad_scale) columns_out<T, V, TPR>(dsc, sums, t, group, C, out + Q_S * plane);
+  if (p.grad_pre_weight) columns_out<T, V, TPR>(dw2, sums, t, group, C, out + Q_W2 * plane);
+  if (p.grad_pre_bias) columns_out<T, V, TPR>(db2, sums, t, group, C, out + Q_B2 * plane);
 }
 
 // The workgroups' column sums added: 16 columns a workgroup, its 64 rows of lanes every 64th part.
@@ -475,18 +482,6 @@ bool norm_sizes_ok(const fx_residual_norm* p) {
          (p->wdtype == FX_F32 || p->wdtype == p->dtype) && (p->gc == 0 || p->gc == 1) && !(p->flags & ~7);
 }
 
-// Rows of all tensors 16-byte aligned: their vectors can be loaded whole.
-bool norm_vectors(const fx_residual_norm& p) {
-  const int64_t v = 16 / (int64_t)dtype_size(p.dtype);
-  uintptr_t ptrs = 0;
-  for (const void* q : {p.x, p.h, p.gc ? p.gate : nullptr, (const void*)p.y, (const void*)p.z, p.grad_y, p.grad_z,
-                        (const void*)p.grad_x, (const void*)p.grad_h, p.gc ? (const void*)p.grad_gate : nullptr})
-    ptrs |= (uintptr_t)q;
-  int64_t strides = p.columns | p.xs | p.xr | p.hs | p.hr | p.os | p.or_;
-  if (p.gate && p.gc) strides |= p.gs | p.gr;
-  return !(ptrs & 15) && strides % v == 0;
-}
-
 bool norm_pointers_ok(const fx_residual_norm& p) {
   const size_t e = dtype_size(p.dtype), w = dtype_size(p.wdtype);
   for (const void* q : {p.x, p.h, p.gate, (const void*)p.y, (const void*)p.z, p.grad_y, p.grad_z,
@@ -499,26 +494,36 @@ bool norm_pointers_ok(const fx_residual_norm& p) {
   return p.x && p.h && aligned(p.stats, 16);
 }
 
-// f(lanes of a row, elements of a lane, whole vectors)
-template <class F>
-void norm_shape(int columns, bool vect, F&& f) {
-  auto go = [&](auto tpr, auto ept) {
-    if (vect)
-      f(tpr, ept, ic<1>{});
-    else
-      f(tpr, ept, ic<0>{});
+// Whether some row is not 16-byte aligned.
+bool norm_loose(const fx_residual_norm& p) {
+  const int64_t v = 16 / (int64_t)dtype_size(p.dtype);
+  uintptr_t ptrs = 0;
+  for (const void* q : {p.x, p.h, p.gc ? p.gate : nullptr, (const void*)p.y, (const void*)p.z, p.grad_y, p.grad_z,
+                        (const void*)p.grad_x, (const void*)p.grad_h, p.gc ? (const void*)p.grad_gate : nullptr})
+    ptrs |= (uintptr_t)q;
+  int64_t strides = p.columns | p.xs | p.xr | p.hs | p.hr | p.os | p.or_;
+  if (p.gate && p.gc) strides |= p.gs | p.gr;
+  return (ptrs & 15) || strides % v;
+}
+
+// f(elements of a vector, lanes of a row)
+template <class T, class F>
+void norm_shape(const fx_residual_norm& p, F&& f) {
+  auto by_lanes = [&](auto v) {
+    switch (norm_tpr(p.columns)) {
+      case 8: return f(v, ic<8>{});
+      case 16: return f(v, ic<16>{});
+      case 32: return f(v, ic<32>{});
+      case 64: return f(v, ic<64>{});
+      case 128: return f(v, ic<128>{});
+      case 256: return f(v, ic<256>{});
+      case 512: return f(v, ic<512>{});
+      default: return f(v, ic<1024>{});
+    }
   };
-  switch (norm_tpr(columns)) {
-    case 8: return go(ic<8>{}, ic<8>{});
-    case 16: return go(ic<16>{}, ic<8>{});
-    case 32: return go(ic<32>{}, ic<8>{});
-    case 64: return go(ic<64>{}, ic<8>{});
-    case 128: return go(ic<128>{}, ic<8>{});
-    case 256: return go(ic<256>{}, ic<8>{});
-    case 512: return go(ic<512>{}, ic<8>{});
-    default:
-      return go(ic<1024>{}, ic<8>{});
-  }
+  if constexpr (sizeof(T) == 4)
+    if (norm_loose(p)) return by_lanes(ic<1>{});
+  by_lanes(ic<VEC16<T>>{});
 }
 
 }  // namespace
@@ -538,11 +543,10 @@ int fx_residual_norm_forward(const fx_residual_norm* p, fx_stream_t stream) {
   a.p = *p;
   return with_type<false>(p->dtype, [&](auto t) {
     using T = decltype(t);
-    norm_shape(p->columns, norm_vectors(*p), [&](auto tpr, auto ept, auto vect) {
-      constexpr int TPR = decltype(tpr)::value, NT = norm_threads(TPR);
+    norm_shape<T>(*p, [&](auto v, auto tpr) {
+      constexpr int V = decltype(v)::value, TPR = decltype(tpr)::value, NT = norm_threads(TPR);
       const int64_t most = cdiv(p->samples * p->rows, NT / TPR), fit = 256 * 2048 / NT;
-      hipLaunchKernelGGL((norm_kernel<T, TPR, decltype(ept)::value, decltype(vect)::value != 0>),
-                         dim3((unsigned)(most < fit ? most : fit)), dim3(NT), 0, (hipStream_t)stream, a);
+      hipLaunchKernelGGL((norm_kernel<T, V, TPR>), dim3((unsigned)(most < fit ? most : fit)), dim3(NT), 0, (hipStream_t)stream, a);
     });
     return launched();
   });
@@ -575,14 +579,13 @@ int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t wor
   return with_type<false>(p->dtype, [&](auto t) {
     using T = decltype(t);
     if (!none) {
-      norm_shape(p->columns, norm_vectors(*p), [&](auto tpr, auto ept, auto vect) {
-        constexpr int TPR = decltype(tpr)::value, EPT = decltype(ept)::value;
-        constexpr bool VECT = decltype(vect)::value != 0;
+      norm_shape<T>(*p, [&](auto v, auto tpr) {
+        constexpr int V = decltype(v)::value, TPR = decltype(tpr)::value;
         const dim3 grid((unsigned)n.groups), block(norm_threads(TPR));
         if ((p->flags & FX_NORM_LAYER) || p->post_bias || p->pre_bias)
-          hipLaunchKernelGGL((norm_grad_kernel<T, TPR, EPT, VECT, true>), grid, block, 0, s, a);
+          hipLaunchKernelGGL((norm_grad_kernel<T, V, TPR, true>), grid, block, 0, s, a);
         else
-          hipLaunchKernelGGL((norm_grad_kernel<T, TPR, EPT, VECT, false>), grid, block, 0, s, a);
+          hipLaunchKernelGGL((norm_grad_kernel<T, V, TPR, false>), grid, block, 0, s, a);
       });
       if (launched() != FX_OK) return FX_ERR_LAUNCH;
     }
