@@ -186,25 +186,31 @@ struct RowFrags {
 
 // acc += (rows row0 .. row0 + 31 of the tile, row0 a multiple of 16) x (the wave's rows): the tile's rows are the accumulator's.
 template <class T, int DP>
-__device__ __forceinline__ v16f row_product(const T* tile, int row0, const RowFrags<T, DP>& b, v16f acc, int lane) {
+__device__ __forceinline__ v16f row_product(const T* tile, int row0, const RowFrags<T, DP>& b, v16f acc, int lane,
+                                            int dim) {
   using M = Mma<T>;
   const T* p = tile + row0 * Tile<T, DP>::STRIDE + Tile<T, DP>::at(lane & 31, (M::KS / 2) * (lane >> 5));
 #pragma unroll
-  for (int s = 0; s < RowFrags<T, DP>::STEPS; ++s)
+  for (int s = 0; s < RowFrags<T, DP>::STEPS; ++s) {
+    if (sizeof(T) == 4 && M::KS * s >= dim) break;  // float32's products take eight times as long as the branch
     acc = M::mma(*reinterpret_cast<const typename M::frag*>(p + M::KS * s), b.f[s], acc);
+  }
   return acc;
 }
 
 // acc[d] += (columns 32 d .. of the tile's rows row0 .. row0 + 31, transposed) x p, contracted over the rows.
 template <class T, int DP>
-__device__ __forceinline__ void column_product(const T* tile, int row0, const v16f& p, v16f (&acc)[DP / 32], int lane) {
+__device__ __forceinline__ void column_product(const T* tile, int row0, const v16f& p, v16f (&acc)[DP / 32], int lane,
+                                               int dim) {
   using M = Mma<T>;
 #pragma unroll
   for (int s = 0; s < 32 / M::KS; ++s) {
     const typename M::frag b = M::from_acc(p, s);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d) {
+      if (sizeof(T) == 4 && 32 * d >= dim) break;
       acc[d] = M::mma(M::template columns<DP>(tile, row0 + M::KS * s, 32 * d, lane), b, acc[d]);
+    }
   }
 }
 

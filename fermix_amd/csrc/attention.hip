@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = bias_block<GEN>(p, bv, kv, kb, k0, qpos, half, far);
-      s[kb] = row_product<T, DP>(kt, 32 * kb, q, s[kb], lane);
+      s[kb] = row_product<T, DP>(kt, 32 * kb, q, s[kb], lane, p.dim);
       if (edge) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + acc_row(i) < left ? s[kb][i] : -INFINITY;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
       for (int d = 0; d < DB; ++d) o[d] *= keep;
     }
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) column_product<T, DP>(vt, 32 * kb, s[kb], o, lane);
+    for (int kb = 0; kb < 2; ++kb) column_product<T, DP>(vt, 32 * kb, s[kb], o, lane, p.dim);
   }
 
   const bool out_in = qi < p.nq;

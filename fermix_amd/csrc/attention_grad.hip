@@ -25,7 +25,7 @@ constexpr size_t tiles_lds() {
 }
 // WAVES: of a workgroup.
 template <class T, int DP, bool GEN, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 128 || WAVES == 8 ? 2 : 1) void attention_dq_kernel(
+__global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 128 && WAVES == 4) ? 2 : 1) void attention_dq_kernel(
     const AttArgs a) {
   constexpr int NT = 64 * WAVES;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -110,8 +110,8 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 128 || WAVES == 
 #pragma unroll 1  // both blocks at once spill at DP = 128: 1269 us at 2 x 16 x 8192 queries, one by one 1120
     for (int kb = 0; kb < 2; ++kb) {
       v16f s = bias_block<GEN>(p, bv, kv, kb, k0, qpos, half, far);
-      s = row_product<T, DP>(kt, 32 * kb, q, s, lane);
-      v16f dp = row_product<T, DP>(vt, 32 * kb, g, v16f{}, lane);
+      s = row_product<T, DP>(kt, 32 * kb, q, s, lane, p.dim);
+      v16f dp = row_product<T, DP>(vt, 32 * kb, g, v16f{}, lane, p.dim);
       if (exact) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i] - ml.x, a.c, -ml.y));
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 128 || WAVES == 
         for (int i = 0; i < 16; ++i) sums.all += dp[i];
       }
       if (p.grad_table) bucket_add<GEN, WEIGHTS>(bv, kv, sums, dp, s, kb, k0, qpos, half, far);
-      column_product<T, DP>(kt, 32 * kb, dp, dq, lane);
+      column_product<T, DP>(kt, 32 * kb, dp, dq, lane, p.dim);
     }
   }
   store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
@@ -204,9 +204,9 @@ __device__ __forceinline__ v16f bias_block_t(const BiasView& bv, const QueryView
 
 // Four waves have 32 keys each. SPLIT: eight do, the first four for dv and the others for dk of the same keys; both
 // form the scores (five products for four), but neither has to hold the other's sums, so that two waves fit a
-// SIMD where the rows are long.
+// SIMD where the rows are long. (Not for float32, whose products take longest: 204 us for 175 at 48 x 302.)
 template <class T, int DP, bool GEN, bool SPLIT>
-__global__ __launch_bounds__(SPLIT ? 512 : 256, DP * (int)sizeof(T) <= 128 || SPLIT ? 2 : 1) void attention_dkv_kernel(
+__global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 : 1) void attention_dkv_kernel(
     const AttArgs a) {
   constexpr int NT = SPLIT ? 512 : 256;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, DP * (int)sizeof(T) <= 128 || SP
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) {
         v16f s = bias_block_t<GEN>(bv, qv, qb, p.offset + q0, kpos, half, far);
-        s = row_product<T, DP>(qt, 32 * qb, k, s, lane);
+        s = row_product<T, DP>(qt, 32 * qb, k, s, lane, p.dim);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int at4 = 32 * qb + 8 * g + 4 * half;
@@ -308,9 +308,9 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, DP * (int)sizeof(T) <= 128 || SP
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = in ? s[i] : 0.0f;
         }
-        if (do_v) column_product<T, DP>(gt, 32 * qb, s, sum[SPLIT ? 0 : 1], lane);
+        if (do_v) column_product<T, DP>(gt, 32 * qb, s, sum[SPLIT ? 0 : 1], lane, p.dim);
         if (!do_k) continue;
-        const v16f dp = row_product<T, DP>(gt, 32 * qb, v, v16f{}, lane);
+        const v16f dp = row_product<T, DP>(gt, 32 * qb, v, v16f{}, lane, p.dim);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 delta = *reinterpret_cast<const float4*>(qv.delta + 32 * qb + 8 * g + 4 * half);
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, DP * (int)sizeof(T) <= 128 || SP
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[4 * g + r] *= dp[4 * g + r] - de[r];
         }
-        column_product<T, DP>(qt, 32 * qb, s, sum[0], lane);
+        column_product<T, DP>(qt, 32 * qb, s, sum[0], lane, p.dim);
       }
     }
   }

@@ -102,8 +102,8 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
     const int k0 = kb / 2 * ATT_TILE;
     const KeyView kv{kpos + k0, kok + kb / 2};
     s[kb] = bias_block<GEN>(p, bv, kv, kb & 1, k0, qpos, half, far[kb / 2]);
-    s[kb] = row_product<T, DP>(t0, 32 * kb, q, s[kb], lane);
-    dp[kb] = row_product<T, DP>(t1, 32 * kb, g, dp[kb], lane);
+    s[kb] = row_product<T, DP>(t0, 32 * kb, q, s[kb], lane, p.dim);
+    dp[kb] = row_product<T, DP>(t1, 32 * kb, g, dp[kb], lane, p.dim);
     if (exact) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i] - ml.x, a.c, -ml.y));
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
     const int k0 = kb / 2 * ATT_TILE;
     if (p.grad_table)
       bucket_add<GEN, false>(bv, KeyView{kpos + k0, nullptr}, sums, dp[kb], s[kb], kb & 1, k0, qpos, half, far[kb / 2]);
-    column_product<T, DP>(t0, 32 * kb, dp[kb], dq, lane);
+    column_product<T, DP>(t0, 32 * kb, dp[kb], dq, lane, p.dim);
   }
   store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
   if (!GEN && p.grad_table) add_pair(sums.ds, bv.map[0], sums.far_ds[0], bv.map[2 * p.radius + 128], sums.far_ds[1]);
