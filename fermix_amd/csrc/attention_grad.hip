@@ -282,7 +282,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
       const bool edge = p.causal && (int64_t)p.offset + q0 < kw + 31;
       const int far = GEN ? 0 : far_side(kw - (p.offset + q0), 32, ATT_TILE, p.radius);
       const bool exact = sizeof(T) == 4 || *qv.exact;
-#pragma unroll
+#pragma unroll sizeof(T) == 4 && DP == 128 ? 1 : 2  // (both blocks at once do not fit the registers there)
       for (int qb = 0; qb < 2; ++qb) {
         v16f s = bias_block_t<GEN>(bv, qv, qb, p.offset + q0, kpos, half, far);
         s = row_product<T, DP>(qt, 32 * qb, k, s, lane, p.dim);

@@ -182,29 +182,28 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, causal, offset, scale):
-    a = _lib.FxAttention()
-    a.batch, a.nq, a.heads, a.dim = q.shape
-    a.nk, a.kv_heads = k.shape[1], k.shape[2]
-    a.dtype, a.causal, a.offset, a.scale = _TYPES[q.dtype], causal, offset, scale
-    a.q, a.k, a.v = _ptr(q), _ptr(k), _ptr(v)
-    a.qb, a.qn, a.qh, _ = q.stride()
-    a.kb, a.kn, a.kh, _ = k.stride()
-    a.vb, a.vn, a.vh, _ = v.stride()
-    if table is not None:
-        a.table, a.map, a.radius, a.buckets = _ptr(table), _ptr(buckets), buckets.numel() // 2, table.shape[0]
-    a.q_pos, a.k_pos, a.lengths, a.q_lengths, a.mask = (_ptr(x) for x in (q_pos, k_pos, lengths, q_lengths, mask))
-    return a
+def _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, causal, offset, scale, out, stats):
+    B, N, H, D = q.shape
+    K, Hkv = k.shape[1], k.shape[2]
+    qb, qn, qh, _ = q.stride()
+    kb, kn, kh, _ = k.stride()
+    vb, vn, vh, _ = v.stride()
+    radius, count = (0, 0) if table is None else (buckets.shape[0] // 2, table.shape[0])
+    return _lib.FxAttention(
+        B, N, K, H, Hkv, D, _TYPES[q.dtype], causal, offset, radius, count, scale,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, qn, qh, kb, kn, kh, vb, vn, vh,
+        _ptr(table), _ptr(buckets), _ptr(q_pos), _ptr(k_pos), _ptr(lengths), _ptr(q_lengths), _ptr(mask),
+        out.data_ptr(), _ptr(stats),
+    )
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, *rest):
-        a = _attention_args(q, k, v, table, *rest)
         B, N, H, D = q.shape
         out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
         stats = torch.empty((B, H, N, 2), dtype=torch.float32, device=q.device)
-        a.out, a.stats = _ptr(out), _ptr(stats)
+        a = _attention_args(q, k, v, table, *rest, out, stats)
         _call("fx_attention_forward", q, ctypes.byref(a))
         buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain = rest
         ctx.save_for_backward(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats)
@@ -214,11 +213,11 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats = ctx.saved_tensors
-        a = _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain)
+        a = _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain, out, stats)
         grad = grad.contiguous()
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         dt = torch.empty_like(table) if ctx.needs_input_grad[3] else None
-        a.out, a.stats, a.grad_out = _ptr(out), _ptr(stats), _ptr(grad)
+        a.grad_out = _ptr(grad)
         a.grad_q, a.grad_k, a.grad_v, a.grad_table = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt)
         ws, wsb = _workspace(lib().fx_attention_grad_workspace(ctypes.byref(a)), q.device)
         _call("fx_attention_grad", q, ctypes.byref(a), _ptr(ws), wsb)
@@ -299,10 +298,8 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     rest = (buckets, q_pos, k_pos, lengths, q_lengths, mask, bool(causal), offset, scale)
     if _wants_grad(q, k, v, table):
         return _Attention.apply(q, k, v, table, *rest)
-    a = _attention_args(q, k, v, table, *rest)
     out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
-    a.out = _ptr(out)
-    _call("fx_attention_forward", q, ctypes.byref(a))
+    _call("fx_attention_forward", q, ctypes.byref(_attention_args(q, k, v, table, *rest, out, None)))
     return out
 
 
@@ -344,19 +341,16 @@ def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table
     _on_device(q)
     if _wants_grad(q, k_cache, v_cache, k, v, table):
         raise NotImplementedError("attention_step has no gradient: call it under torch.no_grad(), or train with attention")
-    a = _lib.FxAttentionStep()
     q, pages, lengths = q.contiguous(), _int32(pages), _int32(lengths)
     k, v = (None if x is None else x.contiguous() for x in (k, v))
-    a.batch, a.heads, a.kv_heads, a.dim, a.dtype = B, H, Hkv, D, _TYPES[q.dtype]
-    a.pages, a.page_size, a.max_pages, a.scale = P, page, pages.shape[1], scale
-    a.q, a.k, a.v, a.k_cache, a.v_cache = _ptr(q), _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache)
-    a.page_table, a.lengths = _ptr(pages), _ptr(lengths)
-    if table is not None:
-        a.table, a.map, a.radius, a.buckets = _ptr(table), _ptr(buckets), buckets.numel() // 2, table.shape[0]
     out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
-    a.out = _ptr(out)
-    ws, wsb = _workspace(lib().fx_attention_step_workspace(ctypes.byref(a)), q.device)
-    _call("fx_attention_step_run", q, ctypes.byref(a), _ptr(ws), wsb)
+    radius, count = (0, 0) if table is None else (buckets.shape[0] // 2, table.shape[0])
+    a = ctypes.byref(_lib.FxAttentionStep(
+        B, H, Hkv, D, _TYPES[q.dtype], P, page, pages.shape[1], radius, count, scale, q.data_ptr(), _ptr(k), _ptr(v),
+        k_cache.data_ptr(), v_cache.data_ptr(), pages.data_ptr(), lengths.data_ptr(), _ptr(table), _ptr(buckets), out.data_ptr(),
+    ))
+    ws, wsb = _workspace(lib().fx_attention_step_workspace(a), q.device)
+    _call("fx_attention_step_run", q, a, _ptr(ws), wsb)
     return out
 
 
@@ -395,33 +389,27 @@ def _gate_view(gate, x):
     )
 
 
-def _norm_args(x, h, gate, columns, alpha, eps, flags):
+def _norm_args(x, h, gate, columns, alpha, eps, flags, y=None, z=None, stats=None):
     """x, h contiguous."""
-    a = _lib.FxResidualNorm()
     C = x.shape[-1]
-    S, R, swapped, (a.gs, a.gr, a.gc) = _gate_view(gate, x)
-    a.samples, a.rows, a.columns = S, R, C
+    S, R, swapped, (gs, gr, gc) = _gate_view(gate, x)
     # rows of x: sample s, row r is row s R + r, or r S + s where the samples are the inner dimension
-    for s, r in (("xs", "xr"), ("hs", "hr"), ("os", "or_")):
-        setattr(a, s, C if swapped else R * C)
-        setattr(a, r, S * C if swapped else C)
+    s, r = (C, S * C) if swapped else (R * C, C)
     wide = next((t.dtype for t in columns if t is not None), torch.float32)
-    a.dtype, a.wdtype, a.flags, a.eps, a.alpha = _TYPES[x.dtype], _TYPES[wide], flags, eps, alpha
-    a.x, a.h, a.gate = _ptr(x), _ptr(h), _ptr(gate)
-    for name, t in zip(_COLUMNS, columns):
-        setattr(a, name, _ptr(t))
-    return a
+    return _lib.FxResidualNorm(
+        S, R, C, _TYPES[x.dtype], _TYPES[wide], flags, eps, alpha, x.data_ptr(), h.data_ptr(), _ptr(gate), s, r, s, r, gs, gr, gc,
+        s, r, *(_ptr(t) for t in columns), _ptr(y), _ptr(z), _ptr(stats),
+    )
 
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, gate, post_weight, post_bias, scale, pre_weight, pre_bias, alpha, eps, flags):
         columns = (post_weight, post_bias, scale, pre_weight, pre_bias)
-        a = _norm_args(x, h, gate, columns, alpha, eps, flags)
         stats = torch.empty(x.shape[:-1] + (4,), dtype=torch.float32, device=x.device)
         y = torch.empty_like(x)
         z = torch.empty_like(x) if flags & FX_NORM_PRE else None
-        a.y, a.z, a.stats = _ptr(y), _ptr(z), _ptr(stats)
+        a = _norm_args(x, h, gate, columns, alpha, eps, flags, y, z, stats)
         _call("fx_residual_norm_forward", x, ctypes.byref(a))
         ctx.save_for_backward(x, h, gate, stats, *columns)
         ctx.plain = alpha, eps, flags
@@ -434,14 +422,14 @@ class _ResidualNorm(torch.autograd.Function):
         if grad_y is None and grad_z is None:
             return (None,) * 11
         x, h, gate, stats, *columns = ctx.saved_tensors
-        a = _norm_args(x, h, gate, columns, *ctx.plain)
+        a = _norm_args(x, h, gate, columns, *ctx.plain, stats=stats)
         grad_y, grad_z = (None if g is None else g.contiguous() for g in (grad_y, grad_z))
         dx, dh = torch.empty_like(x), torch.empty_like(h)
         dgate = None if gate is None else torch.empty_like(gate)
         dcolumns = [
             torch.empty_like(t) if t is not None and need else None for t, need in zip(columns, ctx.needs_input_grad[3:8])
         ]
-        a.stats, a.grad_y, a.grad_z = _ptr(stats), _ptr(grad_y), _ptr(grad_z)
+        a.grad_y, a.grad_z = _ptr(grad_y), _ptr(grad_z)
         a.grad_x, a.grad_h, a.grad_gate = _ptr(dx), _ptr(dh), _ptr(dgate)
         for name, t in zip(_COLUMNS, dcolumns):
             setattr(a, "grad_" + name, _ptr(t))
@@ -504,11 +492,9 @@ def residual_norm(x, h, *, post_weight=None, post_bias=None, gate=None, scale=No
     x, h = x.contiguous(), h.contiguous()
     if _wants_grad(x, h, gate, *columns):
         return _ResidualNorm.apply(x, h, gate, *columns, alpha, float(eps), flags)
-    a = _norm_args(x, h, gate, columns, alpha, float(eps), flags)
     y = torch.empty_like(x)
     z = torch.empty_like(x) if pre_norm else None
-    a.y, a.z = _ptr(y), _ptr(z)
-    _call("fx_residual_norm_forward", x, ctypes.byref(a))
+    _call("fx_residual_norm_forward", x, ctypes.byref(_norm_args(x, h, gate, columns, alpha, float(eps), flags, y, z)))
     return (y, z) if pre_norm else y
 
 
