@@ -6,17 +6,19 @@
 // The lanes of a row add up its scores for all the heads that share it; each row position of the wave keeps a
 // running maximum and sum of its own, joined at the end by lane moves.
 //
+// Heads that share K and V, 16-bit types (step_mma_kernel): up to sixteen heads are the columns of 16 x 16 products,
+// S^T = K q^T with K straight from memory, then O^T = V^T P^T with V through LDS of the wave's own for its column
+// reads; a lane has one head's scores of eight tokens in registers. Whatever the heads, the work is that of one pass.
+//
 // With many samples a wave takes a kv head of a sample by itself. With few, four waves take it together, and
 // where that is not enough either its tokens are split over workgroups (as evenly as the sample's own length
 // allows), whose sums a second launch joins. The order of all sums depends on sizes and lengths alone.
-#include "net.h"
+#include "attention.h"
 
 namespace fx {
 namespace net {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float F32_MAX = 3.402823466e38f;
 constexpr int STEP_WAVES = 4, STEP_NT = 64 * STEP_WAVES;
 
 struct StepArgs {
@@ -27,6 +29,7 @@ struct StepArgs {
   int shift;
   float* part;      // [batch][heads][splits][dim]
   float2* stat;     // [batch][heads][splits]: maximum and sum
+  int sums_bytes, stat_at;  // step_mma_kernel's LDS: the V tiles (then the waves' sums, statistics at stat_at)
 };
 
 // A bias in units of log2 e; finite entries stay finite.
@@ -321,6 +324,241 @@ __global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
   }
 }
 
+typedef float v4f_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4f_t mma16(vec_t<__bf16, 8> a, vec_t<__bf16, 8> b, v4f_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f_t mma16(vec_t<_Float16, 8> a, vec_t<_Float16, 8> b, v4f_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int STEP_TOKENS = 32, STEP_HEADS = 16;
+
+// Lane l = 16 g + c. K operand: token c (and 16 + c), elements 32 s + 8 g ..; scores: head c, tokens 4 g + r and
+// 16 + 4 g + r; these, rounded, are the second product's operand; V is stored as Tile has it and read by columns.
+template <class T, int DP, int W>
+__global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) {
+  constexpr int KS = DP / 32, DB = DP / 16, S = Tile<T, DP>::STRIDE;
+  using V8 = vec_t<T, 8>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const fx_attention_step& p = a.p;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  T* const vt = reinterpret_cast<T*>(smem) + wave * STEP_TOKENS * S;  // [token][dim]
+  float* const tabs = reinterpret_cast<float*>(smem + a.sums_bytes);  // [unit][bucket][STEP_HEADS]
+  unsigned char* const map = reinterpret_cast<unsigned char*>(tabs + (W == 1 ? STEP_WAVES : 1) * STEP_HEADS * p.buckets);
+  float* const tab = tabs + (W == 1 ? wave : 0) * STEP_HEADS * p.buckets;
+
+  const int group = p.heads / p.kv_heads, blocks = (group + STEP_HEADS - 1) / STEP_HEADS, units = p.kv_heads * blocks;
+  const int at_unit = W == 1 ? (int)blockIdx.y * STEP_WAVES + wave : (int)blockIdx.y, unit = min(units - 1, at_unit);
+  const bool spare = at_unit >= units;  // a wave without a unit
+  const int kh = unit / blocks, h0 = kh * group + (unit % blocks) * STEP_HEADS;
+  const int heads = min(STEP_HEADS, group - (unit % blocks) * STEP_HEADS);
+  const int split = blockIdx.x;
+  const int64_t b = blockIdx.z;
+  const int len = p.lengths[b];
+  const int n = p.k ? (len < 0 ? 0 : len == 0x7fffffff ? len : len + 1) : max(len, 0);  // tokens attended to
+  const bool over = (int64_t)n > (int64_t)p.max_pages * p.page_size;
+  int per = (int)(((int64_t)n + a.splits - 1) / a.splits);
+  per = (int)min((int64_t)n, ((int64_t)per + a.unit - 1) / a.unit * a.unit);
+  const int64_t t0 = (int64_t)split * per, t1 = over ? 0 : min((int64_t)n, t0 + per);
+  const int64_t row0 = (b * p.heads + h0) * a.splits + split;
+  if (t0 >= t1 && a.splits > 1 && !over) {
+    if ((int)threadIdx.x < heads) a.stat[row0 + (int64_t)threadIdx.x * a.splits] = make_float2(-INFINITY, 0.0f);
+    return;
+  }
+
+  const int64_t row_size = (int64_t)p.kv_heads * p.dim;
+  const T* const kc = static_cast<const T*>(p.k_cache) + (int64_t)kh * p.dim;
+  const T* const vc = static_cast<const T*>(p.v_cache) + (int64_t)kh * p.dim;
+  const int64_t new_row = (b * p.kv_heads + kh) * p.dim;
+  const int* const table = p.page_table + b * p.max_pages;
+  bool bad = over;
+  V8 k[2][KS], v[2][KS];
+  int64_t slot[2];
+  // the next tokens' places: slot >= 0 in the cache; -1 no token; -2 a page outside the cache
+  auto find = [&](int64_t base) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t at = base + 16 * t + c;
+      slot[t] = -1;
+      if (at < t1) {
+        const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)at * a.magic) >> a.shift);
+        const int page = table[pg];
+        slot[t] = -2;
+        if ((uint32_t)page < (uint64_t)p.pages)
+          slot[t] = ((int64_t)page * p.page_size + ((uint32_t)at - pg * (uint32_t)p.page_size)) * row_size;
+        else
+          bad = true;
+      }
+    }
+  };
+  // their rows; the new token's are in the call, and go into the cache (by the kv head's first heads)
+  auto fetch = [&](int64_t base) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bool fresh = p.k && base + 16 * t + c == n - 1;
+      const T* ks = fresh ? static_cast<const T*>(p.k) + new_row : kc + slot[t];
+      const T* vs = fresh ? static_cast<const T*>(p.v) + new_row : vc + slot[t];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        k[t][s] = v[t][s] = {};
+        if (slot[t] >= 0) {
+          k[t][s] = load_part<T>(ks, 32 * s + 8 * g, p.dim, a.vec);
+          v[t][s] = load_part<T>(vs, 32 * s + 8 * g, p.dim, a.vec);
+        }
+      }
+      if (fresh && slot[t] >= 0 && unit % blocks == 0 && !spare) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int d = 32 * s + 8 * g + e;
+            if (d < p.dim) {
+              static_cast<T*>(p.k_cache)[slot[t] + (int64_t)kh * p.dim + d] = k[t][s][e];
+              static_cast<T*>(p.v_cache)[slot[t] + (int64_t)kh * p.dim + d] = v[t][s][e];
+            }
+          }
+      }
+    }
+  };
+  constexpr int STRIDE = W * STEP_TOKENS;
+  const int64_t first = t0 + (W == 1 ? 0 : wave * STEP_TOKENS);
+  find(first);
+  fetch(first);
+  V8 q[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    q[s] = {};
+    if (c < heads)
+      q[s] = load_part<T>(static_cast<const T*>(p.q) + (b * p.heads + h0 + c) * p.dim, 32 * s + 8 * g, p.dim, false);
+  }
+  if (p.table) {
+    const int at = W == 1 ? lane : threadIdx.x, nt = W == 1 ? 64 : STEP_NT;
+    for (int i = at; i < STEP_HEADS * p.buckets; i += nt) {
+      const int h = i % STEP_HEADS;
+      tab[i] = h < heads ? log2_bias(p.table[(int64_t)(i / STEP_HEADS) * p.heads + h0 + h]) : 0.0f;
+    }
+    for (int i = threadIdx.x; i <= p.radius; i += STEP_NT) map[i] = (unsigned char)min((int)p.map[i], p.buckets - 1);
+  }
+  __syncthreads();
+
+  const float scale = p.scale * LOG2E;
+  float m = -INFINITY, l = 0.0f;
+  v4f_t o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = v4f_t{};
+  const float far = p.table ? tab[STEP_HEADS * map[0] + c] : 0.0f;
+  for (int64_t base = first; base < t1; base += STRIDE) {
+    // V into the wave's own tile, as in Tile::at; K's products
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        *reinterpret_cast<V8*>(vt + Tile<T, DP>::at(16 * t + c, 32 * s + 8 * g)) = v[t][s];
+    v4f_t s[2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < KS; ++i) s[t] = mma16(k[t][i], q[i], s[t]);
+    find(base + STRIDE);
+    if (base + STRIDE < t1) fetch(base + STRIDE);
+
+    float top = -INFINITY;
+    const bool near = p.table && base + STEP_TOKENS - 1 - (n - 1) > -p.radius;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t at = base + 16 * t + 4 * g + r;
+        float bias = far;
+        if (near) bias = tab[STEP_HEADS * map[max((int)min(at - (n - 1), (int64_t)0), -p.radius) + p.radius] + c];
+        s[t][r] = at < t1 ? __builtin_fmaf(s[t][r], scale, bias) : -INFINITY;
+        top = fmaxf(top, s[t][r]);
+      }
+    const float next = fmaxf(m, join32<MaxOp>(join16<MaxOp>(top)));
+    const float ref = next == -INFINITY ? 0.0f : next;
+    const float keep = __builtin_amdgcn_exp2f(m - ref);
+    m = next;
+    V8 w;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float x = __builtin_amdgcn_exp2f(s[t][r] - ref);
+        sum += x;
+        w[4 * t + r] = (T)x;
+      }
+    l = l * keep + sum;
+    if (__any(keep != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= keep;
+    }
+    // tokens 4 g + 0..3 and 16 on, one column a lane
+    const T* const col = vt + (g + 4 * (c >> 2)) * S + 4 * (c & 3);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const s16x4 x = read_columns4(col + 16 * d), y = read_columns4(col + 16 * S + 16 * d);
+      o[d] = mma16(__builtin_bit_cast(V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), w, o[d]);
+    }
+  }
+  l = join32<AddOp>(join16<AddOp>(l));
+
+  if constexpr (W == 1) {
+    bad = __any(bad);
+    if (spare || c >= heads) return;
+    const float inv = bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+    T* const out = static_cast<T*>(p.out) + (b * p.heads + h0 + c) * p.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      vec_t<T, 4> x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = (T)(o[d][r] * inv);
+      if (a.vec) {
+        if (16 * d + 4 * g < p.dim) *reinterpret_cast<vec_t<T, 4>*>(out + 16 * d + 4 * g) = x;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * d + 4 * g + r < p.dim) out[16 * d + 4 * g + r] = x[r];
+      }
+    }
+  } else {
+    // the waves' sums, in the V tiles' place
+    const bool any_bad = __syncthreads_or(bad);
+    float* const acc_lds = reinterpret_cast<float*>(smem);                      // [wave][head][DP + 1]
+    float2* const stat_lds = reinterpret_cast<float2*>(smem + a.stat_at);       // [wave][head]
+    constexpr int R = DP + 1;
+    if (c < heads) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc_lds[(wave * heads + c) * R + 16 * d + 4 * g + r] = o[d][r];
+      if (g == 0) stat_lds[wave * heads + c] = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * DP; i += STEP_NT) {
+      const int h = i / DP, d = i % DP;
+      float top = -INFINITY, sum = 0.0f, x = 0.0f;
+      for (int w = 0; w < W; ++w) top = fmaxf(top, stat_lds[w * heads + h].x);
+      for (int w = 0; w < W; ++w) {
+        const float2 st = stat_lds[w * heads + h];
+        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
+        sum += f * st.y;
+        x += f * acc_lds[(w * heads + h) * R + d];
+      }
+      if (any_bad) x = sum = NAN;
+      if (d >= p.dim) continue;
+      if (a.splits == 1) {
+        static_cast<T*>(p.out)[(b * p.heads + h0 + h) * p.dim + d] = (T)(sum == 0.0f ? 0.0f : x / sum);
+      } else {
+        const int64_t r = row0 + (int64_t)h * a.splits;
+        a.part[r * p.dim + d] = x;
+        if (d == 0) a.stat[r] = make_float2(any_bad ? NAN : top, sum);
+      }
+    }
+  }
+}
+
 // One (sample, head) a workgroup: the parts' weights by the first wave, then each lane a column of a share of the
 // parts, the shares joined in order.
 template <class T>
@@ -377,7 +615,14 @@ bool step_sizes_ok(const fx_attention_step* p) {
                   : p->buckets == 0 && p->radius == 0;
 }
 
-int step_heads(int group) { return group >= 3 ? 4 : group; }  // heads that a workgroup takes at once
+// Whether the heads that share K and V are the columns of a product. (One head by itself is not worth it.)
+bool step_mma(const fx_attention_step& p) { return p.dtype != FX_F32 && p.heads > p.kv_heads; }
+
+// Heads that a unit takes at once.
+int step_heads(const fx_attention_step& p) {
+  const int group = p.heads / p.kv_heads;
+  return step_mma(p) ? STEP_HEADS : group >= 3 ? 4 : group;
+}
 
 // Units (samples x kv heads x blocks of their heads) from which each gets one wave: four waves a SIMD of the card.
 constexpr int64_t STEP_ALONE = 4096;
@@ -385,8 +630,7 @@ constexpr int64_t STEP_ALONE = 4096;
 // Parts of a sample's tokens: enough workgroups for the card, none under 256 tokens of the longest sample
 // that the table can hold.
 int step_splits(const fx_attention_step& p) {
-  const int group = p.heads / p.kv_heads;
-  const int64_t rows = p.batch * p.kv_heads * cdiv(group, step_heads(group));
+  const int64_t rows = p.batch * p.kv_heads * cdiv(p.heads / p.kv_heads, step_heads(p));
   const int64_t want = cdiv(1024, rows), most = cdiv((int64_t)p.max_pages * p.page_size, 256);
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s);
@@ -427,7 +671,7 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
   const int splits = step_splits(*p);
   if (splits > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < fx_attention_step_workspace(p)))
     return FX_ERR_WORKSPACE;
-  const int group = p->heads / p->kv_heads, per = step_heads(group);
+  const int group = p->heads / p->kv_heads, per = step_heads(*p);
   const int64_t rows = p->kv_heads * cdiv(group, per);
   const bool alone = p->batch * rows >= STEP_ALONE;
   if (rows > 65535 || (int64_t)p->max_pages * p->page_size > 0x7fffffff) return FX_ERR_UNSUPPORTED;
@@ -478,6 +722,35 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
         else
           go(dp, ic<4>{});
       };
+      if constexpr (sizeof(T) == 2) {
+        if (step_mma(*p)) {
+          auto mma = [&](auto dp) {
+            constexpr int DP = decltype(dp)::value;
+            const int tiles = STEP_WAVES * STEP_TOKENS * Tile<T, DP>::STRIDE * (int)sizeof(T);
+            c.stat_at = STEP_WAVES * STEP_HEADS * (DP + 1) * 4;
+            const int sums = alone ? 0 : c.stat_at + STEP_WAVES * STEP_HEADS * 8;
+            c.sums_bytes = (int)cdiv(tiles > sums ? tiles : sums, 16) * 16;
+            const size_t lds = c.sums_bytes + 4 * (size_t)(alone ? STEP_WAVES : 1) * STEP_HEADS * p->buckets + p->radius + 1;
+            if (alone)
+              hipLaunchKernelGGL((step_mma_kernel<T, DP, 1>), dim3(1, (unsigned)cdiv(rows, STEP_WAVES), (unsigned)nb),
+                                 dim3(STEP_NT), lds, s, c);
+            else
+              hipLaunchKernelGGL((step_mma_kernel<T, DP, STEP_WAVES>), dim3(splits, (unsigned)rows, (unsigned)nb),
+                                 dim3(STEP_NT), lds, s, c);
+          };
+          if (p->dim <= 32)
+            mma(ic<32>{});
+          else if (p->dim <= 64)
+            mma(ic<64>{});
+          else
+            mma(ic<128>{});
+          if (launched() != FX_OK) return FX_ERR_LAUNCH;
+          if (splits > 1)
+            hipLaunchKernelGGL((step_join_kernel<T>), dim3((unsigned)(nb * p->heads)), dim3(STEP_NT),
+                               sizeof(float) * (splits + STEP_NT), s, c);
+          continue;
+        }
+      }
       if (p->dim <= 16)
         by_heads(ic<16>{});
       else if (p->dim <= 32)

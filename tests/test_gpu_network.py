@@ -338,6 +338,17 @@ def test_step(dev, dtype, lengths, H, Hkv, D, page, M):
     check_step({**c, "table": None, "buckets": None, "scale": 0.3}, dev, dtype, "no bias")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("B,H,Hkv,D", [(700, 6, 6, 32), (1100, 8, 4, 40), (2100, 6, 2, 64), (4200, 2, 1, 128)])
+def test_step_many_units(dev, dtype, B, H, Hkv, D):
+    """Enough samples and kv heads that each gets a wave of its own, in numbers that leave some waves spare."""
+    gen = torch.Generator().manual_seed(B)
+    lengths = torch.randint(-1, 60, (B,), generator=gen).tolist()
+    c = step_case(gen, dtype, lengths, H, Hkv, D, 13, 5, 16, 12)
+    c["pages"][7, 0] = -5
+    check_step(c, dev, dtype)
+
+
 def test_step_many_samples(dev):
     """More samples than a grid dimension holds, one token each of a small cache."""
     B = 66000
