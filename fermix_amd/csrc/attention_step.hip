@@ -25,8 +25,9 @@ struct StepArgs {
   fx_attention_step p;
   int splits, vec;
   int unit;         // a part's tokens are a multiple of this
-  uint32_t magic;   // token / page_size = (token magic) >> shift for tokens below 2^31
+  uint32_t magic;   // token / page_size = the high word of token magic, >> shift, for tokens below 2^31 (page_size > 1)
   int shift;
+  uint32_t row_size, page_elements;
   float* part;      // [batch][heads][splits][dim]
   float2* stat;     // [batch][heads][splits]: maximum and sum
   int sums_bytes, stat_at;  // step_mma_kernel's LDS: the V tiles (then the waves' sums, statistics at stat_at)
@@ -36,6 +37,15 @@ struct StepArgs {
 __device__ __forceinline__ float log2_bias(float b) {
   const float x = b * LOG2E;
   return isinf(b) || !(fabsf(x) > F32_MAX) ? x : copysignf(F32_MAX, b);
+}
+
+// First element of a token's row in the cache, -1 for a page outside it: three 32-bit products (a 64-bit address
+// calculation for each token costs as much as the token's scores).
+__device__ __forceinline__ int64_t token_slot(const StepArgs& a, const int* pages, uint32_t t) {
+  const uint32_t pg = a.p.page_size == 1 ? t : __umulhi(t, a.magic) >> a.shift;
+  const uint32_t page = (uint32_t)pages[pg];
+  if ((uint64_t)page >= (uint64_t)a.p.pages) return -1;
+  return (int64_t)((uint64_t)page * a.page_elements + (t - pg * (uint32_t)a.p.page_size) * a.row_size);
 }
 
 template <int V, class T>
@@ -62,7 +72,7 @@ __device__ __forceinline__ vec_t<T, VEC16<T>> load_part(const T* row, int d0, in
 // G: heads at a time. W: waves that share a unit (a block of G heads of a kv head of a sample), 1 or 4.
 template <class T, int DP, int G, int W>
 __global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
-  constexpr int V = VEC16<T>, LPT = DP / V, ROWS = 64 / LPT, U = 4, STRIDE = W * ROWS * U;
+  constexpr int V = VEC16<T>, LPT = DP / V, ROWS = 64 / LPT, U = W == 1 ? 2 : 4, STRIDE = W * ROWS * U;
   extern __shared__ __align__(16) unsigned char smem[];
   const fx_attention_step& p = a.p;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = W == 1 ? wave : 0;
@@ -82,7 +92,8 @@ __global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
   const bool over = (int64_t)n > (int64_t)p.max_pages * p.page_size;
   int per = (int)(((int64_t)n + a.splits - 1) / a.splits);
   per = (int)min((int64_t)n, ((int64_t)per + a.unit - 1) / a.unit * a.unit);
-  const int64_t t0 = (int64_t)split * per, t1 = over ? 0 : min((int64_t)n, t0 + per);
+  // tokens from here on in 32 bits: all are below 2^31, and what is added to them is small
+  const uint32_t t0 = (uint32_t)min((int64_t)n, (int64_t)split * per), t1 = over ? 0u : (uint32_t)min((int64_t)n, (int64_t)t0 + per);
   const int64_t row0 = (b * p.heads + h0) * a.splits + split;
   const int part = lane % LPT, d0 = part * V, row = lane / LPT;
   if (t0 >= t1 && a.splits > 1 && !over) {
@@ -90,30 +101,22 @@ __global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
     return;
   }
 
-  const bool own = p.k && t1 == n && n > 0;  // this part has the new token, which is in the call, not the cache
-  const int64_t end = own ? t1 - 1 : t1;     // of the cached tokens
-  const int64_t row_size = (int64_t)p.kv_heads * p.dim;
+  const bool own = p.k && t1 == (uint32_t)n && n > 0;  // this part has the new token, which is in the call, not the cache
+  const uint32_t end = own ? t1 - 1 : t1;              // of the cached tokens
   const T* const kc = static_cast<const T*>(p.k_cache) + (int64_t)kh * p.dim;
   const T* const vc = static_cast<const T*>(p.v_cache) + (int64_t)kh * p.dim;
   const int* const table = p.page_table + b * p.max_pages;
   bool bad = over;
-  // where a token's row is, in elements; -1 for a page outside the cache
-  auto slot_of = [&](int64_t t) -> int64_t {
-    const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)t * a.magic) >> a.shift);
-    const int page = table[pg];
-    if ((uint32_t)page >= (uint64_t)p.pages) return -1;
-    return ((int64_t)page * p.page_size + ((uint32_t)t - pg * (uint32_t)p.page_size)) * row_size;
-  };
-  const int64_t first = t0 + (W == 1 ? 0 : wave * ROWS * U);
+  const uint32_t first = t0 + (W == 1 ? 0 : wave * ROWS * U);
   int64_t slot[U];
   vec_t<T, V> k[U], v[U], nk[U], nv[U];
-  auto find = [&](int64_t base) {
+  auto find = [&](uint32_t base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t t = base + u * ROWS + row;
+      const uint32_t t = base + u * ROWS + row;
       slot[u] = -1;
       if (t < end) {
-        slot[u] = slot_of(t);
+        slot[u] = token_slot(a, table, t);
         if (slot[u] < 0) bad = true;
       }
     }
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
     const int64_t at = (b * p.kv_heads + kh) * p.dim;
     const vec_t<T, V> xk = load_part<T>(static_cast<const T*>(p.k) + at, d0, p.dim, false);
     const vec_t<T, V> xv = load_part<T>(static_cast<const T*>(p.v) + at, d0, p.dim, false);
-    const int64_t to = slot_of(n - 1);
+    const int64_t to = token_slot(a, table, n - 1);
     if (to < 0) bad = true;
     if (W == 1 || wave == 0) {
       if (to >= 0 && unit % blocks == 0 && row == 0) {
@@ -195,7 +198,7 @@ __global__ __launch_bounds__(STEP_NT, 3) void step_kernel(const StepArgs a) {
     }
   }
 
-  for (int64_t base = first; base < end; base += STRIDE) {
+  for (uint32_t base = first; base < end; base += STRIDE) {
     if (W > 1) {
       fetch(nk, nv);
       find(base + 2 * STRIDE);
@@ -360,14 +363,14 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
   const bool over = (int64_t)n > (int64_t)p.max_pages * p.page_size;
   int per = (int)(((int64_t)n + a.splits - 1) / a.splits);
   per = (int)min((int64_t)n, ((int64_t)per + a.unit - 1) / a.unit * a.unit);
-  const int64_t t0 = (int64_t)split * per, t1 = over ? 0 : min((int64_t)n, t0 + per);
+  // tokens from here on in 32 bits: all are below 2^31, and what is added to them is small
+  const uint32_t t0 = (uint32_t)min((int64_t)n, (int64_t)split * per), t1 = over ? 0u : (uint32_t)min((int64_t)n, (int64_t)t0 + per);
   const int64_t row0 = (b * p.heads + h0) * a.splits + split;
   if (t0 >= t1 && a.splits > 1 && !over) {
     if ((int)threadIdx.x < heads) a.stat[row0 + (int64_t)threadIdx.x * a.splits] = make_float2(-INFINITY, 0.0f);
     return;
   }
 
-  const int64_t row_size = (int64_t)p.kv_heads * p.dim;
   const T* const kc = static_cast<const T*>(p.k_cache) + (int64_t)kh * p.dim;
   const T* const vc = static_cast<const T*>(p.v_cache) + (int64_t)kh * p.dim;
   const int64_t new_row = (b * p.kv_heads + kh) * p.dim;
@@ -375,28 +378,23 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
   bool bad = over;
   V8 k[2][KS], v[2][KS];
   int64_t slot[2];
-  // the next tokens' places: slot >= 0 in the cache; -1 no token; -2 a page outside the cache
-  auto find = [&](int64_t base) {
+  // the next tokens' places in the cache; -1 without one
+  auto find = [&](uint32_t base) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int64_t at = base + 16 * t + c;
+      const uint32_t at = base + 16 * t + c;
       slot[t] = -1;
       if (at < t1) {
-        const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)at * a.magic) >> a.shift);
-        const int page = table[pg];
-        slot[t] = -2;
-        if ((uint32_t)page < (uint64_t)p.pages)
-          slot[t] = ((int64_t)page * p.page_size + ((uint32_t)at - pg * (uint32_t)p.page_size)) * row_size;
-        else
-          bad = true;
+        slot[t] = token_slot(a, table, at);
+        if (slot[t] < 0) bad = true;
       }
     }
   };
   // their rows; the new token's are in the call, and go into the cache (by the kv head's first heads)
-  auto fetch = [&](int64_t base) {
+  auto fetch = [&](uint32_t base) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const bool fresh = p.k && base + 16 * t + c == n - 1;
+      const bool fresh = p.k && base + 16 * t + c == (uint32_t)n - 1;
       const T* ks = fresh ? static_cast<const T*>(p.k) + new_row : kc + slot[t];
       const T* vs = fresh ? static_cast<const T*>(p.v) + new_row : vc + slot[t];
 #pragma unroll
@@ -422,7 +420,7 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
     }
   };
   constexpr int STRIDE = W * STEP_TOKENS;
-  const int64_t first = t0 + (W == 1 ? 0 : wave * STEP_TOKENS);
+  const uint32_t first = t0 + (W == 1 ? 0 : wave * STEP_TOKENS);
   find(first);
   fetch(first);
   V8 q[KS];
@@ -448,7 +446,7 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = v4f_t{};
   const float far = p.table ? tab[STEP_HEADS * map[0] + c] : 0.0f;
-  for (int64_t base = first; base < t1; base += STRIDE) {
+  for (uint32_t base = first; base < t1; base += STRIDE) {
     // V into the wave's own tile, as in Tile::at; K's products
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -464,14 +462,14 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
     if (base + STRIDE < t1) fetch(base + STRIDE);
 
     float top = -INFINITY;
-    const bool near = p.table && base + STEP_TOKENS - 1 - (n - 1) > -p.radius;
+    const bool near = p.table && (int)(base + STEP_TOKENS) - n > -p.radius;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t at = base + 16 * t + 4 * g + r;
+        const uint32_t at = base + 16 * t + 4 * g + r;
         float bias = far;
-        if (near) bias = tab[STEP_HEADS * map[max((int)min(at - (n - 1), (int64_t)0), -p.radius) + p.radius] + c];
+        if (near) bias = tab[STEP_HEADS * map[max(min((int)at - (n - 1), 0), -p.radius) + p.radius] + c];
         s[t][r] = at < t1 ? __builtin_fmaf(s[t][r], scale, bias) : -INFINITY;
         top = fmaxf(top, s[t][r]);
       }
@@ -615,7 +613,8 @@ bool step_sizes_ok(const fx_attention_step* p) {
                   : p->buckets == 0 && p->radius == 0;
 }
 
-// Whether the heads that share K and V are the columns of a product. (One head by itself is not worth it.)
+// Whether the heads that share K and V are the columns of a product. (With one head fifteen columns are idle: 167 us for
+// 128 at 4096 samples of 8 heads, up to 128 tokens, head dimension 32.)
 bool step_mma(const fx_attention_step& p) { return p.dtype != FX_F32 && p.heads > p.kv_heads; }
 
 // Heads that a unit takes at once.
@@ -674,7 +673,9 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
   const int group = p->heads / p->kv_heads, per = step_heads(*p);
   const int64_t rows = p->kv_heads * cdiv(group, per);
   const bool alone = p->batch * rows >= STEP_ALONE;
-  if (rows > 65535 || (int64_t)p->max_pages * p->page_size > 0x7fffffff) return FX_ERR_UNSUPPORTED;
+  if (rows > 65535 || (int64_t)p->max_pages * p->page_size > 0x7fffff00 ||
+      (int64_t)p->kv_heads * p->dim * p->page_size > 0xffffffffll)
+    return FX_ERR_UNSUPPORTED;
 
   StepArgs a{};
   a.p = *p;
@@ -682,10 +683,13 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
   a.unit = 64;
   a.vec = p->dim % (16 / (int)e) == 0 && aligned(p->k_cache, 16) && aligned(p->v_cache, 16) && aligned(p->k, 16) &&
           aligned(p->v, 16) && aligned(p->out, 16);
-  int bits = 0;  // ceil(log2 page_size)
+  // token / page_size for tokens below 2^31: ceil(2^(31 + bits) / page_size) has 32 bits, bits = ceil(log2 page_size)
+  int bits = 0;
   while ((1ll << bits) < p->page_size) ++bits;
-  a.shift = 31 + bits;
-  a.magic = (uint32_t)(((1ull << a.shift) + p->page_size - 1) / p->page_size);
+  a.shift = bits - 1;
+  a.magic = (uint32_t)(((1ull << (31 + bits)) + p->page_size - 1) / p->page_size);
+  a.row_size = (uint32_t)p->kv_heads * p->dim;
+  a.page_elements = (uint32_t)((int64_t)a.row_size * p->page_size);
   a.part = static_cast<float*>(workspace);
   a.stat = reinterpret_cast<float2*>(a.part + step_part_floats(*p, splits));
   const hipStream_t s = (hipStream_t)stream;
