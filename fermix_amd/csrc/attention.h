@@ -408,6 +408,26 @@ int attention_shape(const fx_attention& p, F&& f) {
 
 // ------------------------------------------------------------------ gradient
 
+// Buckets of a block's pairs (as bias_block has them).
+template <bool GEN>
+__device__ __forceinline__ void buckets_of(const BiasView& bv, const KeyView& kv, int kb, int k0, int qpos, int half,
+                                           int (&t)[16]) {
+  if constexpr (GEN) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int4 kp = *reinterpret_cast<const int4*>(kv.pos + 32 * kb + 8 * g + 4 * half);
+      const int k[4] = {kp.x, kp.y, kp.z, kp.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[4 * g + r] = distance_bucket(bv.map, bv.radius, k[r], qpos);
+    }
+  } else {
+    const int d = max(-(bv.radius + 64), min(bv.radius, k0 - qpos));
+    const unsigned char* l = bv.map + d + bv.radius + 64 + 32 * kb + 4 * half;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = l[acc_row(i)];
+  }
+}
+
 // The lane's bucket sums: of dS, of its query's P (WEIGHTS: the 16-bit types), and what tiles past the
 // radius add to the first and the last distance's bucket.
 struct Sums {
@@ -433,24 +453,8 @@ __device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv
     }
     return;
   }
-  // all lookups before the first add: the compiler keeps a read that follows one behind it
-  int t[16];
-  if constexpr (GEN) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int4 kp = *reinterpret_cast<const int4*>(kv.pos + 32 * kb + 8 * g + 4 * half);
-      const int k[4] = {kp.x, kp.y, kp.z, kp.w};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        t[4 * g + r] = distance_bucket(bv.map, bv.radius, k[r], qpos);
-      }
-    }
-  } else {
-    const int d = max(-(bv.radius + 64), min(bv.radius, k0 - qpos));
-    const unsigned char* l = bv.map + d + bv.radius + 64 + 32 * kb + 4 * half;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = l[acc_row(i)];
-  }
+  int t[16];  // all lookups before the first add: the compiler keeps a read that follows one behind it
+  buckets_of<GEN>(bv, kv, kb, k0, qpos, half, t);
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
     add_pair(sums.ds, t[i], ds[i], t[i + 1], ds[i + 1]);

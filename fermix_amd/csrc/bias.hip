@@ -126,16 +126,23 @@ __global__ __launch_bounds__(64 * W) void bias_grad_kernel(const BiasArgs a) {
     load_keys<V>(a.k_pos + b * a.nk + key, k);
     const int* qp = a.q_pos + b * a.nq;
     const T* g = static_cast<const T*>(a.table) + (b * a.heads + h) * a.nq * (int64_t)a.nk + key;
-    for (int i = first; i < end; i += BIAS_UNROLL * step) {
-      vec_t<T, V> x[BIAS_UNROLL];
-      int q[BIAS_UNROLL];
+    vec_t<T, V> x[BIAS_UNROLL], y[BIAS_UNROLL];
+    int q[BIAS_UNROLL], r[BIAS_UNROLL];
+    // rows from i on; a row past the end adds zeros
+    auto fetch = [&](int i, vec_t<T, V>(&to)[BIAS_UNROLL], int(&pos)[BIAS_UNROLL]) {
 #pragma unroll
       for (int u = 0; u < BIAS_UNROLL; ++u) {
-        const int r = i + u * step;
-        x[u] = {};  // a row past the end adds zeros
-        q[u] = qp[min(r, end - 1)];
-        if (r < end) x[u] = *reinterpret_cast<const vec_t<T, V>*>(g + (int64_t)r * a.nk);
+        const int at = i + u * step;
+        to[u] = {};
+        pos[u] = qp[min(at, end - 1)];
+        if (at < end) to[u] = *reinterpret_cast<const vec_t<T, V>*>(g + (int64_t)at * a.nk);
       }
+    };
+    if (first < end) fetch(first, y, r);
+    for (int i = first; i < end; i += BIAS_UNROLL * step) {
+#pragma unroll
+      for (int u = 0; u < BIAS_UNROLL; ++u) x[u] = y[u], q[u] = r[u];
+      if (i + BIAS_UNROLL * step < end) fetch(i + BIAS_UNROLL * step, y, r);  // on their way while these are added
       int t[BIAS_UNROLL * V];
 #pragma unroll
       for (int j = 0; j < BIAS_UNROLL * V; ++j) t[j] = distance_bucket(map, a.radius, k[j % V], q[j / V]);
@@ -174,11 +181,10 @@ __global__ __launch_bounds__(BIAS_NT) void bucket_join_kernel(const A* part, int
 
 int bias_waves(int buckets) { return buckets <= 32 ? 4 : buckets <= 64 ? 2 : 1; }
 
-// Workgroups of a head in the gradient: about what the card holds at once.
+// Workgroups of a head in the gradient: about what the card holds at once, with as many items each.
 int64_t bias_grad_groups(int buckets, int64_t batch, int heads, int nq, int nk, int v) {
-  const int64_t most = Tiling(64 * bias_waves(buckets), batch, nq, nk / v).items;
-  const int64_t fit = cdiv(1280, heads);
-  return most < fit ? most : fit;
+  const int64_t items = Tiling(64 * bias_waves(buckets), batch, nq, nk / v).items;
+  return cdiv(items, cdiv(items, cdiv(1280, heads)));
 }
 
 int bias_vec(int nk, size_t size, const void* p) {
@@ -237,8 +243,11 @@ int fx_relative_bias(const void* table, const uint8_t* map, int32_t radius, int3
 size_t fx_relative_bias_grad_workspace(int32_t buckets, int64_t batch, int32_t heads, int32_t nq, int32_t nk,
                                        int32_t dtype) {
   if (!bias_sizes_ok(0, buckets, batch, heads, nq, nk, dtype) || batch == 0 || nq == 0 || nk == 0) return 0;
-  // of the scalar kernel, which has the most workgroups
-  return (size_t)bias_grad_groups(buckets, batch, heads, nq, nk, 1) * heads * buckets * (dtype == FX_F64 ? 8 : 4);
+  // of whichever way to load has the more workgroups: the pointer decides
+  const int v = (int)(16 / dtype_size(dtype));
+  const int64_t single = bias_grad_groups(buckets, batch, heads, nq, nk, 1);
+  const int64_t whole = nk % v ? 0 : bias_grad_groups(buckets, batch, heads, nq, nk, v);
+  return (size_t)(single > whole ? single : whole) * heads * buckets * (dtype == FX_F64 ? 8 : 4);
 }
 
 int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radius, int32_t buckets,
