@@ -137,7 +137,7 @@ i32: nq nk heads kv_heads dim dtype causal offset radius buckets
 f32: scale
 p: q k v
 i64: qb qn qh kb kn kh vb vn vh
-p: table map q_pos k_pos lengths q_lengths mask out stats grad_out grad_q grad_k grad_v grad_table
+p: table map q_pos k_pos lengths q_lengths mask out out_low stats grad_out grad_q grad_k grad_v grad_table
 """)
 
 FxAttentionStep = _struct("FxAttentionStep", """
@@ -165,6 +165,7 @@ for _n, _s in (("attention", FxAttention), ("residual_norm", FxResidualNorm)):
     SIGNATURES[f"fx_{_n}_forward"] = (ctypes.c_int, [_sp, _p])
     SIGNATURES[f"fx_{_n}_grad_workspace"] = (_sz, [_sp])
     SIGNATURES[f"fx_{_n}_grad"] = (ctypes.c_int, [_sp, _p, _sz, _p])
+SIGNATURES["fx_attention_keeps_low"] = (_i32, [ctypes.POINTER(FxAttention)])
 SIGNATURES.update({
     "fx_relative_bias": (ctypes.c_int, [_p, _p, _i32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p]),
     "fx_relative_bias_grad_workspace": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32]),

@@ -259,6 +259,35 @@ __device__ __forceinline__ void store_rows(T* row, bool in, const v16f (&acc)[DP
     }
 }
 
+// What a rounding to T loses, as float16 of LOW_SCALE times it: with the rounded value 19 bits or more.
+template <class T>
+constexpr float LOW_SCALE = __is_same(T, __bf16) ? 256.0f : 2048.0f;
+
+template <class T, int DP>
+__device__ __forceinline__ void store_low(_Float16* row, bool in, const v16f (&acc)[DP / 32], float f, int dim,
+                                          bool whole, int half) {
+  if (!in) return;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * half;
+      vec_t<_Float16, 4> x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = acc[d][4 * g + r] * f, low = (v - (float)(T)v) * LOW_SCALE<T>;
+        x[r] = (_Float16)fmaxf(-65504.0f, fminf(65504.0f, low));
+      }
+      if (whole) {
+        if (c < dim) *reinterpret_cast<vec_t<_Float16, 4>*>(row + c) = x;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (c + r < dim) row[c + r] = x[r];
+      }
+    }
+}
+
 // Bias of one head. Two forms:
 //  - positions that count up (GEN = false): the bias depends on key - query alone, so LDS holds it laid
 //    out over the distances -(R + 64) .. R + 64, saturated past R. A lane clamps once a tile, and
@@ -313,6 +342,7 @@ struct AttArgs {
   int whole;   // rows are whole 16-byte vectors
   float c;     // scale log2(e)
   float inv_scale;
+  int weights;  // gradient: whether P is summed beside dS
   int tiles;   // items of a head
   int64_t items;
   float* delta;  // gradient: [batch][heads][nq] sum_d out grad_out
@@ -428,7 +458,7 @@ __device__ __forceinline__ void buckets_of(const BiasView& bv, const KeyView& kv
   }
 }
 
-// The lane's bucket sums: of dS, of its query's P (WEIGHTS: the 16-bit types), and what tiles past the
+// The lane's bucket sums: of dS, of its query's P (weights), and what tiles past the
 // radius add to the first and the last distance's bucket.
 struct Sums {
   float* ds;
@@ -439,15 +469,16 @@ struct Sums {
 __device__ __forceinline__ unsigned fixed_weight(float p) { return (unsigned)(p * 0x1p30f); }
 
 // Adds a block's dS and P (rows: keys; column: the lane's query).
-template <bool GEN, bool WEIGHTS>
+template <bool GEN>
 __device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv, Sums& sums, const v16f& ds,
-                                           const v16f& w, int kb, int k0, int qpos, int half, int far) {
+                                           const v16f& w, int kb, int k0, int qpos, int half, int far,
+                                           bool weights) {
   if (!GEN && far) {
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) total += ds[i];
     sums.far_ds[far > 0] += total;
-    if (WEIGHTS) {
+    if (weights) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) sums.far_weight[far > 0] += w[i];
     }
@@ -458,14 +489,15 @@ __device__ __forceinline__ void bucket_add(const BiasView& bv, const KeyView& kv
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
     add_pair(sums.ds, t[i], ds[i], t[i + 1], ds[i + 1]);
-    if (WEIGHTS) {
-      atomicAdd(sums.weight + 32 * t[i], fixed_weight(w[i]));
-      atomicAdd(sums.weight + 32 * t[i + 1], fixed_weight(w[i + 1]));
-    }
+  }
+  if (weights) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) atomicAdd(sums.weight + 32 * t[i], fixed_weight(w[i]));
   }
 }
 
-// The gradient of short sequences in one launch (attention_short.hip): where it applies.
+// The gradient of short sequences (attention_short.hip): where it applies. Where heads share K and V it gives dq, the bucket
+// sums and delta, and the general second launch dk and dv.
 bool attention_grad_short_fits(const fx_attention& p);
 int launch_attention_grad_short(const AttArgs& a, hipStream_t s);
 

@@ -124,6 +124,9 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
   const float inv = l > 0.0f ? 1.0f / l : (l != l ? l : 0.0f);
   const int64_t row = (at.b * p.nq + qi) * p.heads + at.h;
   store_rows<T, DP>(static_cast<T*>(p.out) + row * p.dim, out_in, o, inv, p.dim, a.whole, half);
+  if constexpr (sizeof(T) == 2)
+    if (p.out_low)
+      store_low<T, DP>(static_cast<_Float16*>(p.out_low) + row * p.dim, out_in, o, inv, p.dim, a.whole, half);
   if (p.stats && out_in && half == 0)
     reinterpret_cast<float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi] =
         l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
@@ -148,7 +151,7 @@ bool attention_sizes_ok(const fx_attention* p) {
 bool attention_pointers_ok(const fx_attention& p) {
   const size_t e = dtype_size(p.dtype);
   for (const void* q : {p.q, p.k, p.v, (const void*)p.out, p.grad_out, (const void*)p.grad_q, (const void*)p.grad_k,
-                        (const void*)p.grad_v})
+                        (const void*)p.grad_v, (const void*)p.out_low})
     if (!aligned(q, e)) return false;
   for (const void* q : {(const void*)p.table, (const void*)p.q_pos, (const void*)p.k_pos, (const void*)p.lengths,
                         (const void*)p.q_lengths, (const void*)p.grad_table})
@@ -163,7 +166,7 @@ AttArgs attention_args(const fx_attention& p) {
   const int64_t e = (int64_t)dtype_size(p.dtype), v = 16 / e;
   const int64_t strides = p.dim | p.qb | p.qn | p.qh | p.kb | p.kn | p.kh | p.vb | p.vn | p.vh;
   const uintptr_t in = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.grad_out | (uintptr_t)p.out |
-                       (uintptr_t)p.grad_q | (uintptr_t)p.grad_k | (uintptr_t)p.grad_v;
+                       (uintptr_t)p.out_low | (uintptr_t)p.grad_q | (uintptr_t)p.grad_k | (uintptr_t)p.grad_v;
   a.whole = strides % v == 0 && !(in & 15);
   a.c = p.scale * LOG2E;
   a.inv_scale = 1.0f / p.scale;
@@ -175,6 +178,10 @@ AttArgs attention_args(const fx_attention& p) {
 
 using namespace fx;
 using namespace fx::net;
+
+extern "C" int32_t fx_attention_keeps_low(const fx_attention* p) {
+  return attention_sizes_ok(p) && p->dtype != FX_F32 && !attention_grad_short_fits(*p);
+}
 
 extern "C" int fx_attention_forward(const fx_attention* p, fx_stream_t stream) {
   if (!attention_sizes_ok(p)) return FX_ERR_INVALID_ARGUMENT;

@@ -8,8 +8,8 @@
 //
 // Bucket sums: each lane adds its dS to sums of its own in LDS, [bucket][lane] (no two lanes share a
 // bank or an address, a wave's LDS operations complete in order); tiles past the radius add up in
-// registers; the workgroups' sums are joined by a last launch. For the 16-bit types delta as out gives it is
-// off by what P and out lost to rounding, some 1e-3, which a bucket's sum would keep. A query's dS
+// registers; the workgroups' sums are joined by a last launch. delta as out gives it is off by what P and out lost to
+// rounding (16-bit types: some 1e-3, out_low takes most of it), which a bucket's sum would keep. A query's dS
 // then add up to that error instead of to 0, so the launch also sums P by query and bucket, and takes
 // (sum of the query's dS) x (sum of its P in the bucket) off at the end. As the correction is small, P is summed
 // in fixed point (units of 2^-30), whose order does not matter, the two halves of a wave in one place.
@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
   KeyView kv{reinterpret_cast<int*>(rest), reinterpret_cast<unsigned long long*>(rest + 256)};
   rest += 272;
   const BiasView bv(GEN, rest, p.radius);
-  constexpr bool WEIGHTS = sizeof(T) == 2;
+  const bool weights_on = p.grad_table && (sizeof(T) == 2 || a.weights);
   float* const row_sum = reinterpret_cast<float*>(rest + view_lds(GEN, p.radius));  // [wave][32]
   float* const ds_sums = row_sum + 32 * WAVES;                                             // [wave][bucket][64]
   unsigned* const weights = reinterpret_cast<unsigned*>(ds_sums + 64 * WAVES * p.buckets);  // [wave][bucket][32]
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
   if (p.grad_table)
     for (int t = 0; t < p.buckets; ++t) {
       sums.ds[64 * t] = 0.0f;
-      if (WEIGHTS) sums.weight[32 * t] = 0u;
+      if (weights_on) sums.weight[32 * t] = 0u;
     }
   RowFrags<T, DP> q, g;
   q.load(static_cast<const T*>(p.q) + at.b * p.qb + (int64_t)qi * p.qn + at.h * p.qh, in, p.dim, a.whole, half);
@@ -74,6 +74,18 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
     for (int s = 0; s < RowFrags<T, DP>::STEPS; ++s)
 #pragma unroll
       for (int e = 0; e < M::KS / 2; ++e) delta += (float)o.f[s][e] * (float)g.f[s][e];
+    if constexpr (sizeof(T) == 2) {
+      if (p.out_low) {
+        RowFrags<_Float16, DP> low;
+        low.load(static_cast<const _Float16*>(p.out_low) + row * p.dim, in, p.dim, a.whole, half);
+        float d = 0.0f;
+#pragma unroll
+        for (int s = 0; s < RowFrags<T, DP>::STEPS; ++s)
+#pragma unroll
+          for (int e = 0; e < M::KS / 2; ++e) d += (float)low.f[s][e] * (float)g.f[s][e];
+        delta += d * (1.0f / LOW_SCALE<T>);
+      }
+    }
     delta = half_sum(delta);
   }
   const float2 ml = in ? reinterpret_cast<const float2*>(p.stats)[stat] : make_float2(0.0f, INFINITY);
@@ -130,23 +142,23 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = s[i] * (dp[i] - delta);
-      if (WEIGHTS) {
+      if (sizeof(T) == 2 || weights_on) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sums.all += dp[i];
       }
-      if (p.grad_table) bucket_add<GEN, WEIGHTS>(bv, kv, sums, dp, s, kb, k0, qpos, half, far);
+      if (p.grad_table) bucket_add<GEN>(bv, kv, sums, dp, s, kb, k0, qpos, half, far, weights_on);
       column_product<T, DP>(kt, 32 * kb, dp, dq, lane, p.dim);
     }
   }
   store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
-  // what dS add up to is delta's error (WEIGHTS): the second launch gets delta without it
-  const float all = WEIGHTS ? half_sum(sums.all) : 0.0f;
+  // what dS add up to is delta's error: the second launch gets delta without it
+  const float all = sizeof(T) == 2 || weights_on ? half_sum(sums.all) : 0.0f;
   if (qi < p.nq && half == 0) a.delta[stat] = delta + all;
   if (p.grad_table) {
     if (!GEN) {
       const int t[2] = {bv.map[0], bv.map[2 * p.radius + 128]};
       add_pair(sums.ds, t[0], sums.far_ds[0], t[1], sums.far_ds[1]);
-      for (int i = 0; WEIGHTS && i < 2; ++i) atomicAdd(sums.weight + 32 * t[i], fixed_weight(sums.far_weight[i]));
+      for (int i = 0; weights_on && i < 2; ++i) atomicAdd(sums.weight + 32 * t[i], fixed_weight(sums.far_weight[i]));
     }
     if (half == 0) row_sum[32 * wave + lane] = all;
     __syncthreads();
@@ -156,7 +168,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
       for (int w = 0; w < WAVES; ++w) {
 #pragma unroll 4
         for (int l = 0; l < 64; ++l) x += ds_sums[(w * p.buckets + t) * 64 + ((l + t) & 63)];  // rotated: no shared bank
-        if (WEIGHTS)
+        if (weights_on)
 #pragma unroll 4
           for (int l = 0; l < 32; ++l) {
             const int r = (l + t) & 31;
@@ -327,9 +339,16 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
   if (do_v) store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, sum[SPLIT ? 0 : 1], 1.0f, p.dim, a.whole, half);
 }
 
+// Whether P is summed beside dS. For float32, whose delta is off by float32's roundings only, where these add up over many
+// keys (3000 keys: the bucket sums' error 1.8e-6 without, 0.9e-6 with; at 302 it is 0.7e-6, and 190 us for 133, as
+// the sums leave LDS for one workgroup a CU), and not for rows of 128 with more buckets than LDS holds both for.
+bool sums_weights(const fx_attention& p) {
+  return p.dtype != FX_F32 || (p.nk > 1024 && (p.dim <= 64 || p.buckets <= 32));
+}
+
 // Bytes of a workgroup's bucket sums in the first launch.
 size_t sums_lds(const fx_attention& p, int waves) {
-  return waves * (128 + (p.dtype == FX_F32 ? 256 : 384) * (size_t)p.buckets);
+  return waves * (128 + (sums_weights(p) ? 384 : 256) * (size_t)p.buckets);
 }
 
 // Waves of a workgroup of the first launch: eight where the rows are long (they leave the registers for two waves a
@@ -369,17 +388,17 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
   }
   if (p->nk > 0 && (!p->k || !p->v || !p->grad_k || !p->grad_v)) return FX_ERR_INVALID_ARGUMENT;
   AttArgs a = attention_args(*p);
-  if (attention_grad_short_fits(*p)) {
-    a.part = static_cast<float*>(workspace);
+  a.delta = static_cast<float*>(workspace);
+  a.part = a.delta + delta_floats(*p);
+  a.weights = sums_weights(*p);
+  const bool in_short = attention_grad_short_fits(*p), own = p->heads == p->kv_heads;
+  if (in_short) {
     a.tiles = 1;
     a.items = p->batch * p->heads;
     if (a.items > 0x7fffffff) return FX_ERR_UNSUPPORTED;
     const int st = launch_attention_grad_short(a, s);
-    if (st != FX_OK || !p->grad_table) return st;
-    return launch_bucket_join(a.part, p->batch, p->buckets, p->heads, p->grad_table, s);
+    if (st != FX_OK) return st;
   }
-  a.delta = static_cast<float*>(workspace);
-  a.part = a.delta + delta_floats(*p);
   const int waves = dq_waves(*p), qtiles = (int)cdiv(p->nq, 32 * waves), ktiles = (int)cdiv(p->nk, 128);
   if (p->batch * p->heads * qtiles > 0x7fffffff || p->batch * p->kv_heads * ktiles > 0x7fffffff)
     return FX_ERR_UNSUPPORTED;
@@ -391,7 +410,7 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
     const size_t lds_q = tiles + 272 + view + (p->grad_table ? sums_lds(*p, waves) : 0);
     const size_t lds_kv = tiles + 1040 + view;
     constexpr bool LONG_ROWS = DP == 128 && sizeof(T) == 2;
-    if (qtiles) {
+    if (qtiles && !in_short) {
       a.tiles = qtiles;
       a.items = p->batch * p->heads * qtiles;
       auto go = [&](auto w) {
@@ -408,7 +427,7 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
         go(ic<4>{});
       }
     }
-    if (ktiles) {
+    if (ktiles && !(in_short && own)) {
       a.tiles = ktiles;
       a.items = p->batch * p->kv_heads * ktiles;
       hipLaunchKernelGGL((attention_dkv_kernel<T, DP, GEN, LONG_ROWS>), dim3((unsigned)a.items),

@@ -5,7 +5,7 @@
 // needed: `out` is not read, dS add up to zero, the bucket sums need no correction. dq comes from the
 // wave's own dS; dk and dv contract over all queries: P, then dS, go through LDS, rounded, as [query][key],
 // beside the waves' query and cotangent rows, and a wave takes 32 of the keys. Five products, each tensor read
-// or written once: bound by memory.
+// or written once: bound by memory. Where heads share K and V a second launch forms dk and dv from the exact delta.
 #include "attention.h"
 
 namespace fx {
@@ -21,12 +21,13 @@ constexpr size_t short_tile() {
 }
 
 template <class T, int DP>
-constexpr size_t short_lds(size_t view, int buckets, bool table) {
-  const size_t sums = table ? SHORT_WAVES * 256 * (size_t)buckets : 0, ps = short_tile<T, SHORT>();
+constexpr size_t short_lds(size_t view, int buckets, bool table, bool own) {
+  const size_t sums = table ? SHORT_WAVES * 256 * (size_t)buckets : 0, ps = !own ? 0 : short_tile<T, SHORT>();
   return 2 * short_tile<T, DP>() + 544 + view + (sums > ps ? sums : ps);
 }
 
-template <class T, int DP, bool GEN>
+// OWN: heads have K and V of their own; else dk and dv are left to the launch that adds up those that share them.
+template <class T, int DP, bool GEN, bool OWN>
 __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_grad_kernel(const AttArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   using M = Mma<T>;
@@ -55,8 +56,9 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
   // K and V, 64 rows at a time, and the wave's own rows
   RowFrags<T, DP> q, g;
   {
-    const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + at.h * p.kh;
-    const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + at.h * p.vh;
+    const int kh = OWN ? at.h : at.h / (p.heads / p.kv_heads);
+    const T* kbase = static_cast<const T*>(p.k) + at.b * p.kb + kh * p.kh;
+    const T* vbase = static_cast<const T*>(p.v) + at.b * p.vb + kh * p.vh;
     TileLoad<T, DP, SHORT_NT> kl[2], vl[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -142,7 +144,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
     if (32 * kb >= klen) continue;
     const int k0 = kb / 2 * ATT_TILE;
     if (p.grad_table)
-      bucket_add<GEN, false>(bv, KeyView{kpos + k0, nullptr}, sums, dp[kb], s[kb], kb & 1, k0, qpos, half, far[kb / 2]);
+      bucket_add<GEN>(bv, KeyView{kpos + k0, nullptr}, sums, dp[kb], s[kb], kb & 1, k0, qpos, half, far[kb / 2], false);
     column_product<T, DP>(t0, 32 * kb, dp[kb], dq, lane, p.dim);
   }
   store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
@@ -159,6 +161,11 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
       x = group_sum<SHORT_WAVES>(x);
       if (threadIdx.x % SHORT_WAVES == 0) out[t] = x;
     }
+  }
+
+  if (!OWN) {
+    if (qi < p.nq && half == 0) a.delta[(at.b * p.heads + at.h) * p.nq + qi] = delta;
+    return;
   }
 
   // the wave's rows of q and dO for K and V; P
@@ -209,9 +216,8 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
 
 }  // namespace
 
-// Short sequences whose heads do not share K and V.
 bool attention_grad_short_fits(const fx_attention& p) {
-  return p.dtype != FX_F32 && p.nq >= 1 && p.nq <= SHORT && p.nk >= 1 && p.nk <= SHORT && p.heads == p.kv_heads;
+  return p.dtype != FX_F32 && p.nq >= 1 && p.nq <= SHORT && p.nk >= 1 && p.nk <= SHORT;
 }
 
 int launch_attention_grad_short(const AttArgs& a, hipStream_t s) {
@@ -220,8 +226,13 @@ int launch_attention_grad_short(const AttArgs& a, hipStream_t s) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
-    const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius), p.buckets, p.grad_table != nullptr);
-    hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN>), dim3((unsigned)a.items), dim3(SHORT_NT), lds, s, a);
+    const bool own = p.heads == p.kv_heads;
+    const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius), p.buckets, p.grad_table != nullptr, own);
+    const dim3 grid((unsigned)a.items), block(SHORT_NT);
+    if (own)
+      hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN, true>), grid, block, lds, s, a);
+    else
+      hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN, false>), grid, block, lds, s, a);
   };
   return attention_shape(p, [&](auto t, auto dp, auto gen) {
     if constexpr (sizeof(t) == 2) go(t, dp, gen);

@@ -182,7 +182,8 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, causal, offset, scale, out, stats):
+def _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, causal, offset, scale, out, stats,
+                    low=None):
     B, N, H, D = q.shape
     K, Hkv = k.shape[1], k.shape[2]
     qb, qn, qh, _ = q.stride()
@@ -193,7 +194,7 @@ def _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, m
         B, N, K, H, Hkv, D, _TYPES[q.dtype], causal, offset, radius, count, scale,
         q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, qn, qh, kb, kn, kh, vb, vn, vh,
         _ptr(table), _ptr(buckets), _ptr(q_pos), _ptr(k_pos), _ptr(lengths), _ptr(q_lengths), _ptr(mask),
-        out.data_ptr(), _ptr(stats),
+        out.data_ptr(), _ptr(low), _ptr(stats),
     )
 
 
@@ -204,16 +205,20 @@ class _Attention(torch.autograd.Function):
         out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
         stats = torch.empty((B, H, N, 2), dtype=torch.float32, device=q.device)
         a = _attention_args(q, k, v, table, *rest, out, stats)
+        low = None
+        if lib().fx_attention_keeps_low(ctypes.byref(a)):
+            low = torch.empty((B, N, H, D), dtype=torch.float16, device=q.device)
+            a.out_low = low.data_ptr()
         _call("fx_attention_forward", q, ctypes.byref(a))
         buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain = rest
-        ctx.save_for_backward(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats)
+        ctx.save_for_backward(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats, low)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats = ctx.saved_tensors
-        a = _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain, out, stats)
+        q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats, low = ctx.saved_tensors
+        a = _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain, out, stats, low)
         grad = grad.contiguous()
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
         dt = torch.empty_like(table) if ctx.needs_input_grad[3] else None
@@ -268,7 +273,7 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     1 / sqrt(D).
 
     Differentiable in q, k, v and table. The gradient keeps q, k, v, out and two float32 a query and
-    head."""
+    head; for 16-bit types past 128 queries or keys also what out lost to rounding, as float16."""
     _tensor(q, "q", dtype=_TYPES, dim=4)
     _tensor(k, "k", q, (q.dtype,), 4)
     _tensor(v, "v", q, (q.dtype,), 4)

@@ -504,10 +504,12 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * its entries may be -inf, and entries of float32's lowest value weigh like any other.
  *
  * fx_attention_forward: out and, if given, stats (batch, heads, nq, 2): the largest S / scale and log2
- * of the sum of exp(S - its maximum); 0 and +inf where there is no key.
+ * of the sum of exp(S - its maximum); 0 and +inf where there is no key. With fx_attention_keeps_low(p) != 0 a
+ * gradient wants out_low besides (float16, the shape of out, packed): what out lost to rounding, times 256 (bfloat16)
+ * or 2048 (float16), without which dq has up to 6 % more error (NULL: not written, not read).
  * fx_attention_grad: grad_q, grad_k, grad_v (strides of their own: those of q, k, v in packed
  * tensors) and grad_table (buckets, heads) float32 (NULL to skip) from grad_out (packed), out
- * (packed) and stats. Deterministic: sums are in an order that depends on sizes alone. */
+ * (packed), stats and out_low. Deterministic: sums are in an order that depends on sizes alone. */
 #define FX_MAX_ATTENTION_BUCKETS 64
 typedef struct fx_attention {
   int64_t batch;
@@ -520,12 +522,13 @@ typedef struct fx_attention {
   const uint8_t* map;
   const int32_t *q_pos, *k_pos, *lengths, *q_lengths;
   const uint8_t* mask;
-  void* out;
+  void *out, *out_low;
   float* stats;
   const void* grad_out;
   void *grad_q, *grad_k, *grad_v;
   float* grad_table;
 } fx_attention;
+int32_t fx_attention_keeps_low(const fx_attention* p); /* host only */
 int fx_attention_forward(const fx_attention* p, fx_stream_t stream);
 size_t fx_attention_grad_workspace(const fx_attention* p);
 int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_bytes, fx_stream_t stream);
