@@ -181,6 +181,15 @@ def test_attention(dev, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("shape", [(1, 1100, 1300, 2, 1, 64, "co"), (1, 1030, 1030, 1, 1, 128, "l"), (2, 90, 1500, 3, 3, 40, "mp"), (1, 1300, 70, 2, 1, 16, "")],
+                         ids=lambda s: "-".join(str(x) for x in s))
+def test_attention_long(dev, dtype, shape):
+    """Many tiles, most of them past the radius as a whole; more queries than keys and the reverse."""
+    gen = torch.Generator().manual_seed(sum(shape[:6]))
+    check_attention(attention_case(gen, dtype, *shape[:6], mode=shape[6]), dev, dtype, gen, shape)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("nb,dist", [(4, 2), (64, 2048), (33, 17), (20, 100)])
 def test_attention_buckets(dev, dtype, nb, dist):
     """The table's largest and smallest sizes, near and far tiles, with both kinds of positions."""
