@@ -61,13 +61,24 @@ def _int32(x):
     return x.to(torch.int32).contiguous()
 
 
+def _once(backward):
+    """A backward without a derivative of its own (asking for one raises); the check costs nothing where
+    none can be asked for."""
+    checked = once_differentiable(backward)
+
+    def either(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return either
+
+
 def _wants_grad(*xs):
     return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)
 
 
 def _call(name, device_of, *args):
     """One C entry point on the input's device and its current stream."""
-    if device_of.get_device() == torch.cuda.current_device():
+    if device_of.get_device() == torch._C._cuda_getDevice():
         check(getattr(lib(), name)(*args, _stream(device_of)), name)
     else:
         with torch.cuda.device(device_of.device):
@@ -135,7 +146,7 @@ class _RelativeBias(torch.autograd.Function):
         return _bias_forward(table.contiguous(), buckets, q, k)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         buckets, q, k = ctx.saved_tensors
         nb, H = ctx.shape
@@ -215,7 +226,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, out, stats, low = ctx.saved_tensors
         a = _attention_args(q, k, v, table, buckets, q_pos, k_pos, lengths, q_lengths, mask, *ctx.plain, out, stats, low)
@@ -422,7 +433,7 @@ class _ResidualNorm(torch.autograd.Function):
         return y if z is None else (y, z)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y, grad_z=None):
         if grad_y is None and grad_z is None:
             return (None,) * 11
