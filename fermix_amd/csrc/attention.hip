@@ -5,6 +5,11 @@
 // query's scores in registers: maximum, sum and rescaling need one exchange between the halves, and the
 // rounded weights are the next product's operand as they are (attention.h). K and V tiles of 64 keys
 // go through LDS, the next tile's loads in flight while one is worked on.
+//
+// Bound by vector instructions beside the products (a score costs some nine, an exponential four of them) for long
+// sequences, by memory and the workgroups' latency for short ones. MI355X: causal, 2 x 16 heads x 8192, head dimension
+// 128, bfloat16, 805 us (680 TFLOP/s); 1024 x 8 heads x 128, head dimension 64, 142 us (3.8 TB/s); float32, 48 x 6
+// heads x 302 ragged, 100 us.
 #include "attention.h"
 
 namespace fx {

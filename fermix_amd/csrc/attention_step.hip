@@ -12,7 +12,11 @@
 //
 // With many samples a wave takes a kv head of a sample by itself. With few, four waves take it together, and
 // where that is not enough either its tokens are split over workgroups (as evenly as the sample's own length
-// allows), whose sums a second launch joins. The order of all sums depends on sizes and lengths alone.
+// allows), whose sums a second launch joins.
+//
+// MI355X: 4096 samples x 8 heads, 64 .. 128 tokens, head dimension 32, bfloat16, 118 us (3.3 TB/s, vector instructions
+// half of it); 4 samples of 32 heads on 8, 32768 .. 65536 tokens, head dimension 128, 160 + 10 us (5.0 TB/s; a large
+// copy reaches 5.1); float32, 48 samples of 6 heads on 2, up to 2000 tokens, 26 + 4 us. The order of all sums depends on sizes and lengths alone.
 #include "attention.h"
 
 namespace fx {

@@ -9,6 +9,10 @@
 // the rows that a lane sees, are added over the workgroup's row groups in LDS, and over the
 // workgroups by a second launch, each in a fixed order.
 //
+// MI355X: 4096 x 128 rows of 512, bfloat16, a gate of the sample: 450 us forward (4.8 TB/s; a large copy reaches 5.1),
+// 803 us gradient (4.0 TB/s, half of its time in vector instructions); 2000 x 90 rows of 333, float32, layer norm, a
+// gate per element: 238 us (5.0 TB/s) and 409 us (4.7 TB/s).
+//
 // With c = y - mean (or y), r the reciprocal deviation, n = c r and dn = dz w2, the norm's
 // gradient is r (dn - n mean(n dn) [- mean(dn)]).
 #include "net.h"
