@@ -409,6 +409,64 @@ def test_step_forbidding_table(dev):
             check_step(c, dev, dtype, low)
 
 
+def test_step_long_offsets(dev):
+    """Pages past 2^31 elements of a cache, in both kernels: what the same pages give in a small one."""
+    gen = torch.Generator().manual_seed(9)
+    for H in (8, 16):
+        c = step_case(gen, torch.bfloat16, [150, 190], H, 8, 128, 64, 3, extra=0)
+        a = {n: gpu(x, dev) for n, x in c.items()}
+        want = fx.attention_step(**a)
+        pages = 2**31 // (64 * 8 * 128) + 10
+        far = torch.arange(pages - 6, pages, device=dev)
+        big = dict(a, pages=(a["pages"] + pages - 6).to(torch.int32))
+        for n in ("k_cache", "v_cache"):
+            big[n] = torch.empty(pages, 64, 8, 128, dtype=torch.bfloat16, device=dev)
+            big[n][far] = c[n].to(dev)
+        assert torch.equal(fx.attention_step(**big), want)
+        for n in ("k_cache", "v_cache"):
+            assert torch.equal(big[n][far], a[n])
+        del big
+
+
+def test_attention_long_offsets(dev):
+    """A batch stride past 2^31 elements."""
+    gen = torch.Generator().manual_seed(10)
+    for dtype in (torch.bfloat16, torch.float32):
+        c = attention_case(gen, dtype, 2, 70, 150, 2, 1, 64)
+        a = {n: gpu(x, dev) for n, x in c.items()}
+        want = fx.attention(**a)
+        room = torch.empty(2**31 + 2**16, dtype=dtype, device=dev)
+        for n in "kv":
+            spread = room.as_strided((2, 150, 1, 64), (2**31 - 64, 64, 64, 1))
+            spread.copy_(a[n])
+            assert torch.equal(fx.attention(**{**a, n: spread}), want)
+        del room, spread
+
+
+def test_step_in_a_graph(dev):
+    """A captured step, replayed while the sequence grows: every replay gives what an eager call gives."""
+    gen = torch.Generator().manual_seed(11)
+    for dtype, H in ((torch.bfloat16, 8), (torch.float32, 4)):
+        c = step_case(gen, dtype, [700, 0, 64], H, 2, 64, 16, 64)
+        a = {n: gpu(x, dev) for n, x in c.items()}
+        eager = {n: x.clone() for n, x in a.items()}
+        fx.attention_step(**{n: x.clone() for n, x in a.items()})
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fx.attention_step(**a)
+        for turn in range(4):
+            for n in ("q", "k", "v"):
+                new = rand(gen, *a[n].shape, dtype=dtype).to(dev)
+                a[n].copy_(new)
+                eager[n].copy_(new)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, fx.attention_step(**eager)), turn
+            assert torch.equal(a["k_cache"], eager["k_cache"]) and torch.equal(a["v_cache"], eager["v_cache"])
+            a["lengths"] += 1
+            eager["lengths"] += 1
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_step_follows_attention(dev, dtype):
     """A sequence token by token gives what attention gives it as a whole, to the roundings of both."""
