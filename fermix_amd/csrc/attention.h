@@ -368,14 +368,19 @@ struct KeyView {
   int* pos;                // [64]
   unsigned long long* ok;  // [1]
 };
-// By one wave, lane j for key k0 + j; a barrier follows.
-__device__ __forceinline__ void fill_keys(const fx_attention& p, int64_t b, int k0, int len, const KeyView& kv,
-                                          int lane) {
+// By one wave, lane j for key k0 + j: from memory with the tile's loads, and into LDS with its stores (a barrier follows).
+struct KeyOf {
+  int pos;
+  bool ok;
+};
+__device__ __forceinline__ KeyOf key_of(const fx_attention& p, int64_t b, int k0, int len, int lane) {
   const int j = k0 + lane;
   const bool in = j < len;
-  const bool ok = in && (!p.mask || p.mask[b * p.nk + j]);
-  kv.pos[lane] = !in ? 0 : p.k_pos ? p.k_pos[b * p.nk + j] : j;
-  const unsigned long long m = __ballot(ok);
+  return KeyOf{!in ? 0 : p.k_pos ? p.k_pos[b * p.nk + j] : j, in && (!p.mask || p.mask[b * p.nk + j])};
+}
+__device__ __forceinline__ void put_keys(const KeyOf& key, const KeyView& kv, int lane) {
+  kv.pos[lane] = key.pos;
+  const unsigned long long m = __ballot(key.ok);
   if (lane == 0) *kv.ok = m;
 }
 

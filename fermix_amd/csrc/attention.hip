@@ -58,7 +58,9 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
   float m = -INFINITY, m_base = -INFINITY, l = 0.0f;  // maximum of the raw scores, that times c, sum
 
   TileLoad<T, DP, NT> kl, vl;
+  KeyOf key{};  // of wave 0's lanes (GEN)
   auto fetch = [&](int k0) {
+    if (GEN && wave == 0) key = key_of(p, at.b, k0, klen, lane);
     auto live = [&](int r) { return !GEN || !p.mask || p.mask[at.b * p.nk + k0 + r]; };
     kl.fetch(kbase + (int64_t)k0 * p.kn, p.kn, keys - k0, p.dim, a.whole, live);
     vl.fetch(vbase + (int64_t)k0 * p.vn, p.vn, keys - k0, p.dim, a.whole, live);
@@ -73,7 +75,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
     __syncthreads();
     kl.put(kt);
     vl.put(vt);
-    if (GEN && wave == 0) fill_keys(p, at.b, k0, klen, kv, lane);
+    if (GEN && wave == 0) put_keys(key, kv, lane);
     __syncthreads();
     if (k0 + ATT_TILE < keys) fetch(k0 + ATT_TILE);
     if (k0 > wave_last) continue;

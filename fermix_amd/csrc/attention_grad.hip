@@ -100,7 +100,9 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = v16f{};
   TileLoad<T, DP, NT> kl, vl;
+  KeyOf key{};  // of wave 0's lanes (GEN)
   auto fetch = [&](int k0) {
+    if (GEN && wave == 0) key = key_of(p, at.b, k0, klen, lane);
     auto live = [&](int r) { return !GEN || !p.mask || p.mask[at.b * p.nk + k0 + r]; };
     kl.fetch(kbase + (int64_t)k0 * p.kn, p.kn, keys - k0, p.dim, a.whole, live);
     vl.fetch(vbase + (int64_t)k0 * p.vn, p.vn, keys - k0, p.dim, a.whole, live);
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
     __syncthreads();
     kl.put(kt);
     vl.put(vt);
-    if (GEN && wave == 0) fill_keys(p, at.b, k0, klen, kv, lane);
+    if (GEN && wave == 0) put_keys(key, kv, lane);
     __syncthreads();
     if (k0 + ATT_TILE < keys) fetch(k0 + ATT_TILE);
     if (k0 > wave_last) continue;
@@ -265,7 +267,17 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
     const T* gbase = static_cast<const T*>(p.grad_out) + (at.b * p.nq * p.heads + h) * p.dim;
     const int64_t stat = (at.b * p.heads + h) * p.nq;
     TileLoad<T, DP, NT> ql, gl;
+    float2 ml;  // of query threadIdx.x of the tile: statistics, delta, position
+    float de;
+    int qp = 0;
     auto fetch = [&](int q0) {
+      if (threadIdx.x < ATT_TILE) {
+        const int i = q0 + threadIdx.x;
+        const bool q_in = i < queries;
+        ml = q_in ? reinterpret_cast<const float2*>(p.stats)[stat + i] : make_float2(0.0f, INFINITY);
+        de = q_in ? a.delta[stat + i] : 0.0f;
+        if (GEN) qp = !q_in ? 0 : p.q_pos ? p.q_pos[at.b * p.nq + i] : p.offset + i;
+      }
       auto live = [](int) { return true; };
       ql.fetch(qbase + (int64_t)q0 * p.qn, p.qn, queries - q0, p.dim, a.whole, live);
       gl.fetch(gbase + (int64_t)q0 * p.heads * p.dim, (int64_t)p.heads * p.dim, queries - q0, p.dim, a.whole, live);
@@ -280,15 +292,12 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
       ql.put(qt);
       gl.put(gt);
       if (threadIdx.x < ATT_TILE) {
-        const int i = q0 + threadIdx.x;
-        const bool q_in = i < queries;
-        const float2 ml = q_in ? reinterpret_cast<const float2*>(p.stats)[stat + i] : make_float2(0.0f, INFINITY);
         const bool exact = sizeof(T) == 4 || __any(fabsf(ml.x * a.c) > BASE_MAX);
         qv.max[threadIdx.x] = ml.x;
         qv.log[threadIdx.x] = exact ? ml.y : ml.x * a.c + ml.y;
         if (threadIdx.x == 0) *qv.exact = exact;
-        qv.delta[threadIdx.x] = q_in ? a.delta[stat + i] : 0.0f;
-        if (GEN) qv.pos[threadIdx.x] = !q_in ? 0 : p.q_pos ? p.q_pos[at.b * p.nq + i] : p.offset + i;
+        qv.delta[threadIdx.x] = de;
+        if (GEN) qv.pos[threadIdx.x] = qp;
       }
       __syncthreads();
       if (q0 + ATT_TILE < queries) fetch(q0 + ATT_TILE);

@@ -76,7 +76,8 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
       kl[i].put(t0 + i * ATT_TILE * ST);
       vl[i].put(t1 + i * ATT_TILE * ST);
     }
-    if (GEN && wave < 2) fill_keys(p, at.b, wave * ATT_TILE, klen, KeyView{kpos + wave * ATT_TILE, kok + wave}, lane);
+    if (GEN && wave < 2)
+      put_keys(key_of(p, at.b, wave * ATT_TILE, klen, lane), KeyView{kpos + wave * ATT_TILE, kok + wave}, lane);
   }
   Sums sums{ds_sums + wave * p.buckets * 64 + lane, nullptr, 0.0f, {}, {}};
   if (p.grad_table)
