@@ -8,8 +8,8 @@
 //
 // Bound by vector instructions beside the products (a score costs some nine, an exponential four of them) for long
 // sequences, by memory and the workgroups' latency for short ones. MI355X: causal, 2 x 16 heads x 8192, head dimension
-// 128, bfloat16, 805 us (680 TFLOP/s); 1024 x 8 heads x 128, head dimension 64, 142 us (3.8 TB/s); float32, 48 x 6
-// heads x 302 ragged, 100 us.
+// 128, bfloat16, 817 us (670 TFLOP/s); 1024 x 8 heads x 128, head dimension 64, 138 us (3.9 TB/s); float32, 48 x 6
+// heads x 302 ragged, 94 us.
 #include "attention.h"
 
 namespace fx {

@@ -3,9 +3,9 @@
 //   dq = scale dS k  and the bias' bucket sums of dS     (a workgroup: 128 queries, over the keys),
 //   dv = P^T dO,  dk = scale dS^T q                      (a workgroup: 128 keys, over the queries of
 //                                                         all heads that share them).
-// MI355X: causal, 2 x 16 heads x 8192, head dimension 128, bfloat16, 1133 + 1943 us (450 TFLOP/s of the five products
+// MI355X: causal, 2 x 16 heads x 8192, head dimension 128, bfloat16, 1157 + 1880 us (450 TFLOP/s of the five products
 // that a gradient needs); bound by the waits of two waves a SIMD at the tiles' barriers (products 29 % of the second
-// launch's time, LDS and vector instructions some 30 % each). float32, 48 x 6 heads x 302 ragged, 136 + 169 us.
+// launch's time, LDS and vector instructions some 30 % each). float32, 48 x 6 heads x 302 ragged, 136 + 160 us.
 //
 // Seven products where one launch would need five, but no sum crosses workgroups: nothing is added
 // by atomics in memory, every order is fixed. The first launch also leaves delta for the second.

@@ -5,8 +5,9 @@
 // needed: `out` is not read, dS add up to zero, the bucket sums need no correction. dq comes from the
 // wave's own dS; dk and dv contract over all queries: P, then dS, go through LDS, rounded, as [query][key],
 // beside the waves' query and cotangent rows, and a wave takes 32 of the keys. Five products, each tensor read
-// or written once: 331 us at 1024 x 8 heads x 128, head dimension 64, bfloat16 (2.8 TB/s), where the two launches for
-// long sequences took 680; bound by the latency of its phases, with two workgroups a CU. Where heads share K and V a second launch forms dk and dv from the exact delta.
+// or written once: 316 us at 1024 x 8 heads x 128, head dimension 64, bfloat16 (2.9 TB/s), where the two launches
+// for long sequences took 680; bound by the latency of its phases, with two workgroups a CU. Where heads share K
+// and V a second launch forms dk and dv from the exact delta.
 #include "attention.h"
 
 namespace fx {
