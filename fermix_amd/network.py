@@ -276,7 +276,8 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     q (B, N, H, D), k and v (B, K, Hkv, D), float32, bfloat16 or float16, any strides (D is
     made contiguous if it is not), D <= 128, H a multiple of Hkv: heads h Hkv / H share a key head.
     table (num_buckets, H) float32 (up to 64 buckets) with buckets as for ``relative_bias``, or
-    None for no bias. Positions: q_pos (B, N) and k_pos (B, K), or None: offset + i and j.
+    None for no bias. Positions: q_pos (B, N) and k_pos (B, K), or None: offset + i and j. Positions
+    and lengths are int32, or int64 of its range.
     lengths (B,): keys at or past it are left out; mask (B, K) bool: keys that are False are; both may
     hide anything, NaN and infinities included. causal: query i sees keys j <= offset + i (what is
     hidden by it alone has to be finite). q_lengths (B,): queries at or past it give 0. A query with no key
@@ -322,9 +323,9 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
 def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table=None, buckets=None, scale=None):
     """Attention of one new token of each sample over a paged key-value cache: out (B, H, D).
 
-    q (B, H, D); k_cache and v_cache (P, page, Hkv, D) contiguous; pages (B, M) int32: token t of
-    sample b is token t % page of cache page pages[b, t // page]; lengths (B,) int32: the tokens
-    that a sample has in the cache. With k and v (B, Hkv, D) the new token's are stored as token
+    q (B, H, D); k_cache and v_cache (P, page, Hkv, D) contiguous; pages (B, M): token t of
+    sample b is token t % page of cache page pages[b, t // page]; lengths (B,): the tokens
+    that a sample has in the cache (both int32, or int64 of its range). With k and v (B, Hkv, D) the new token's are stored as token
     lengths[b] (in place; the caller counts lengths up) and its query, at that position, attends
     to tokens 0 .. lengths[b]; a sample of negative length is left out. Without them the query is that
     of the cache's last token. table, buckets and scale as for ``attention``; a key's distance
@@ -367,6 +368,8 @@ def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table
     ))
     ws, wsb = _workspace(lib().fx_attention_step_workspace(a), q.device)
     _call("fx_attention_step_run", q, a, _ptr(ws), wsb)
+    if k is not None:
+        torch.autograd.graph.increment_version((k_cache, v_cache))  # a graph that saved the caches must not use them
     return out
 
 

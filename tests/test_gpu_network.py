@@ -370,6 +370,25 @@ def test_step_many_samples(dev):
     assert torch.equal(out, v) and torch.equal(kc[:, 0], k) and torch.equal(vc[:, 0], v)
 
 
+def test_step_marks_the_caches_as_written(dev):
+    """A graph that saved the caches before a token was appended refuses to go on with the new values."""
+    k, v = (torch.randn(4, 8, 2, 32, device=dev) for _ in range(2))
+    w = torch.ones((), device=dev, requires_grad=True)
+    pages = torch.arange(2, dtype=torch.int32, device=dev)[:, None]
+    lengths = torch.full((2,), 3, dtype=torch.int32, device=dev)
+    q, new = torch.randn(2, 4, 32, device=dev), torch.randn(2, 2, 32, device=dev)
+    for cache in (k, v):
+        y = (cache * w).sum()
+        with torch.no_grad():
+            fx.attention_step(q, k, v, pages, lengths)  # only reads
+        torch.autograd.grad(y, w)
+        y = (cache * w).sum()
+        with torch.no_grad():
+            fx.attention_step(q, k, v, pages, lengths, k=new, v=new)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, w)
+
+
 def test_step_refused_samples(dev):
     """Samples left out (0, nothing stored), past their pages and with a page outside the cache (NaN);
     the rest of the batch as ever. What lies past a sample's tokens may be NaN."""
