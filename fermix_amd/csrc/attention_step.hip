@@ -16,7 +16,9 @@
 //
 // MI355X: 4096 samples x 8 heads, 64 .. 128 tokens, head dimension 32, bfloat16, 118 us (3.3 TB/s, vector instructions
 // half of it); 4 samples of 32 heads on 8, 32768 .. 65536 tokens, head dimension 128, 160 + 10 us (5.0 TB/s; a large
-// copy reaches 5.1); float32, 48 samples of 6 heads on 2, up to 2000 tokens, 26 + 4 us. The order of all sums depends on sizes and lengths alone.
+// copy reaches 5.1); float32, 48 samples of 6 heads on 2, up to 2000 tokens, 26 + 4 us.
+//
+// The order of all sums depends on sizes and lengths alone.
 #include "attention.h"
 
 namespace fx {
