@@ -176,13 +176,16 @@ def relative_bias(table, buckets, q_pos, k_pos):
     if not q.dim() or not k.dim():
         raise ValueError("q_pos and k_pos: expected (..., Q) and (..., K)")
     _on_device(table)
-    lead = torch.broadcast_shapes(q.shape[:-1], k.shape[:-1])
-    q, k = (_int32(x.expand(lead + x.shape[-1:]).reshape(math.prod(lead), x.shape[-1])) for x in (q, k))
+    lead = q.shape[:-1]
+    if len(lead) != 1 or k.shape[:-1] != lead:  # broadcasting takes as long as a small launch
+        lead = torch.broadcast_shapes(lead, k.shape[:-1])
+        q, k = (x.expand(lead + x.shape[-1:]).reshape(math.prod(lead), x.shape[-1]) for x in (q, k))
+    q, k = _int32(q), _int32(k)
     if _wants_grad(table):
         out = _RelativeBias.apply(table, buckets, q, k)
     else:
         out = _bias_forward(table.contiguous(), buckets, q, k)
-    return out.reshape(lead + out.shape[1:])
+    return out if len(lead) == 1 else out.reshape(lead + out.shape[1:])
 
 
 # ------------------------------------------------------------------ attention
