@@ -427,7 +427,8 @@ __global__ __launch_bounds__(JOIN_NT) void columns_join_kernel(const JoinArgs a)
   }
 }
 
-// The gate's gradient of each sample from its items' column sums: per column, or (gc == 0) over them.
+// The gate's gradient of each sample from its items' column sums: per column, or (gc == 0) over them. Zero without
+// items (no rows).
 template <class T>
 __global__ __launch_bounds__(256) void gate_join_kernel(const float* part, int64_t samples, int64_t chunks, int C,
                                                         int gc, T* out) {
@@ -566,6 +567,9 @@ int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t wor
   if (!norm_sizes_ok(p)) return FX_ERR_INVALID_ARGUMENT;
   const hipStream_t s = (hipStream_t)stream;
   const bool none = p->samples == 0 || p->rows == 0;
+  // values (or rows of columns) of a gate that is summed over the rows: there are some even where there are no rows
+  const int64_t gates = !p->gate || p->gr ? 0 : none && !p->gs ? 1 : p->samples;
+  if (gates && (!p->grad_gate || !aligned(p->grad_gate, dtype_size(p->dtype)))) return FX_ERR_INVALID_ARGUMENT;
   if (!none) {
     if (!norm_pointers_ok(*p) || !p->stats || (p->gate && !p->grad_gate)) return FX_ERR_INVALID_ARGUMENT;
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < fx_residual_norm_grad_workspace(p))
@@ -597,10 +601,9 @@ int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t wor
                {p->grad_post_weight, p->grad_post_bias, p->grad_scale, p->grad_pre_weight, p->grad_pre_bias}};
     hipLaunchKernelGGL((columns_join_kernel<T>), dim3((p->columns + JOIN_COLUMNS - 1) / JOIN_COLUMNS, Q_COLUMNS),
                        dim3(JOIN_NT), 0, s, j);
-    if (!none && p->gate && !p->gr)
-      hipLaunchKernelGGL((gate_join_kernel<T>), dim3((unsigned)p->samples, p->gc ? (p->columns + 255) / 256 : 1),
-                         dim3(256), 0, s, a.gate_part, p->samples, n.chunks, p->columns, (int)p->gc,
-                         static_cast<T*>(p->grad_gate));
+    if (gates)
+      hipLaunchKernelGGL((gate_join_kernel<T>), dim3((unsigned)gates, p->gc ? (p->columns + 255) / 256 : 1), dim3(256),
+                         0, s, a.gate_part, gates, n.chunks, p->columns, (int)p->gc, static_cast<T*>(p->grad_gate));
     return launched();
   });
 }
