@@ -22,6 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._diff import _dual
 from ._kernels import _ptr, _stream, _workspace
 from ._lib import FX_MAX_COLUMNS, FX_MAX_RADIUS, FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE, check, lib
 
@@ -74,6 +75,12 @@ def _once(backward):
 
 def _wants_grad(*xs):
     return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)
+
+
+def _refuse_forward_mode(*xs):
+    """A dual tensor that needs no gradient would go to the kernels as its primal and come back without a tangent."""
+    if any(x is not None and _dual(x) for x in xs):
+        raise NotImplementedError("fermix_amd's network operators have no forward mode: differentiate them in reverse mode")
 
 
 def _call(name, device_of, *args):
@@ -175,6 +182,7 @@ def relative_bias(table, buckets, q_pos, k_pos):
     q, k = (_tensor(x, n, table, _INT) for x, n in ((q_pos, "q_pos"), (k_pos, "k_pos")))
     if not q.dim() or not k.dim():
         raise ValueError("q_pos and k_pos: expected (..., Q) and (..., K)")
+    _refuse_forward_mode(table)
     _on_device(table)
     lead = q.shape[:-1]
     if len(lead) != 1 or k.shape[:-1] != lead:  # broadcasting takes as long as a small launch
@@ -311,6 +319,7 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     if not 0 <= offset <= 2**31 - 1 - max(N, K):
         raise ValueError(f"offset: expected 0 to {2**31 - 1 - max(N, K)}, got {offset}")
     scale = _check_scale(scale, D)
+    _refuse_forward_mode(q, k, v, table)
     _on_device(q)
     q, k, v = _rows(q), _rows(k), _rows(v)
     q_pos, k_pos, lengths, q_lengths = (None if x is None else _int32(x) for x in (q_pos, k_pos, lengths, q_lengths))
@@ -358,6 +367,7 @@ def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table
         raise ValueError(f"pages {tuple(pages.shape)} and lengths {tuple(lengths.shape)} do not fit {B} samples")
     table, buckets = _check_bias(table, buckets, H, q)
     scale = _check_scale(scale, D)
+    _refuse_forward_mode(q, k_cache, v_cache, k, v, table)
     _on_device(q)
     if _wants_grad(q, k_cache, v_cache, k, v, table):
         raise NotImplementedError("attention_step has no gradient: call it under torch.no_grad(), or train with attention")
@@ -509,6 +519,7 @@ def residual_norm(x, h, *, post_weight=None, post_bias=None, gate=None, scale=No
         _tensor(gate, "gate", x, (x.dtype,))
         _gate_view(gate, x)
         gate = gate.contiguous()
+    _refuse_forward_mode(x, h, gate, *columns)
     _on_device(x)
     flags = (FX_NORM_LAYER if norm == "layer" else 0) | (FX_NORM_POST if post_norm else 0) | (FX_NORM_PRE if pre_norm else 0)
     x, h = x.contiguous(), h.contiguous()
