@@ -384,10 +384,16 @@ __device__ __forceinline__ void put_keys(const KeyOf& key, const KeyView& kv, in
   if (lane == 0) *kv.ok = m;
 }
 
-// Whether a block of `rows` x `cols` pairs whose first distance (first key - first query) is d lies past the
-// radius as a whole: 1 above, -1 below, 0 neither. Distances run d - (queries - 1) .. d + (keys - 1).
+// Position of query i where positions count up. Saturates for the rows past the last query that fill a tile.
+__device__ __forceinline__ int counted_pos(const fx_attention& p, int i) {
+  return __builtin_elementwise_add_sat(p.offset, i);
+}
+
+// Whether a block of keys x queries pairs whose first distance (first key - first query) is d lies past the
+// radius as a whole: 1 above, -1 below, 0 neither. Distances run d - (queries - 1) .. d + (keys - 1), which may pass
+// the lowest int32 where d does not: the sums are on the radius' side.
 __device__ __forceinline__ int far_side(int d, int keys, int queries, int radius) {
-  return d - (queries - 1) >= radius ? 1 : d + (keys - 1) <= -radius ? -1 : 0;
+  return d >= radius + (queries - 1) ? 1 : d <= -radius - (keys - 1) ? -1 : 0;
 }
 
 // Start of a score block of 32 keys (rows k0 + 32 kb + ..) for the lane's query: the bias.

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
   const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
   const bool in = qi < qlen;
-  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
+  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : counted_pos(p, qi);
   // keys that any query of the workgroup can see
   int keys = q0 < qlen ? klen : 0;
   if (p.causal) keys = (int)min((int64_t)keys, (int64_t)p.offset + min(q0 + 32 * WAVES, qlen));
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
     if (k0 + ATT_TILE < keys) fetch(k0 + ATT_TILE);
     if (k0 > wave_last) continue;
 
-    const int far = GEN ? 0 : far_side(k0 - (p.offset + q0 + 32 * wave), ATT_TILE, 32, p.radius);
+    const int far = GEN ? 0 : far_side(k0 - counted_pos(p, q0 + 32 * wave), ATT_TILE, 32, p.radius);
     v16f s[2];
     float top = -INFINITY;
     // keys of this tile left to the lane, counted from its half's first row
@@ -148,7 +148,8 @@ bool attention_sizes_ok(const fx_attention* p) {
       p->dim < 1 || p->dim > 128)
     return false;
   if (p->dtype != FX_F32 && p->dtype != FX_BF16 && p->dtype != FX_F16) return false;
-  if (!(p->scale > 0.0f) || !(p->scale <= F32_MAX) || p->offset < 0) return false;
+  if (!(p->scale > 0.0f) || !(p->scale <= F32_MAX)) return false;
+  if (p->offset < 0 || p->offset > 0x7fffffff - (p->nq > p->nk ? p->nq : p->nk)) return false;
   if (p->table ? p->buckets < 1 || p->buckets > FX_MAX_ATTENTION_BUCKETS || p->radius < 0 || p->radius > FX_MAX_RADIUS
                : p->buckets != 0 || p->radius != 0)
     return false;

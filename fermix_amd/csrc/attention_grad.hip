@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
   const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
   const bool in = qi < qlen;
-  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
+  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : counted_pos(p, qi);
   int keys = q0 < qlen ? klen : 0;
   if (p.causal) keys = (int)min((int64_t)keys, (int64_t)p.offset + min(q0 + 32 * WAVES, qlen));
   const int kh = at.h / (p.heads / p.kv_heads);
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
     const int left = (int)max((int64_t)0, min((int64_t)ATT_TILE, last - k0)) - 4 * half;
     const bool edge = k0 + ATT_TILE > klen || q0 + 32 * wave + 32 > qlen ||
                       (p.causal && k0 + ATT_TILE - 1 > wave_last - 31);
-    const int far = GEN ? 0 : far_side(k0 - (p.offset + q0 + 32 * wave), ATT_TILE, 32, p.radius);
+    const int far = GEN ? 0 : far_side(k0 - counted_pos(p, q0 + 32 * wave), ATT_TILE, 32, p.radius);
 #pragma unroll 1  // both blocks at once spill at DP = 128: 1269 us at 2 x 16 x 8192 queries, one by one 1120
     for (int kb = 0; kb < 2; ++kb) {
       v16f s = bias_block<GEN>(p, bv, kv, kb, k0, qpos, half, far);
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
       // first row of the tile that sees the lane's key, counted from its half's first row
       const int from = (p.causal ? (int)max((int64_t)0, min((int64_t)ATT_TILE, (int64_t)ki - p.offset - q0)) : 0) - 4 * half;
       const bool edge = p.causal && (int64_t)p.offset + q0 < kw + 31;
-      const int far = GEN ? 0 : far_side(kw - (p.offset + q0), 32, ATT_TILE, p.radius);
+      const int far = GEN ? 0 : far_side(kw - counted_pos(p, q0), 32, ATT_TILE, p.radius);
       const bool exact = sizeof(T) == 4 || *qv.exact;
 #pragma unroll sizeof(T) == 4 && DP == 128 ? 1 : 2  // (both blocks at once do not fit the registers there)
       for (int qb = 0; qb < 2; ++qb) {

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
   const int klen = p.lengths ? max(0, min(p.lengths[at.b], p.nk)) : p.nk;
   const bool in = qi < qlen;
-  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : p.offset + qi;
+  const int qpos = p.q_pos ? (qi < p.nq ? p.q_pos[at.b * p.nq + qi] : 0) : counted_pos(p, qi);
   const int64_t row = (at.b * p.nq + qi) * p.heads + at.h;
 
   // K and V, 64 rows at a time, and the wave's own rows
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
   float delta = 0.0f;
   int far[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) far[i] = GEN ? 0 : far_side(i * ATT_TILE - (p.offset + 32 * wave), ATT_TILE, 32, p.radius);
+  for (int i = 0; i < 2; ++i) far[i] = GEN ? 0 : far_side(i * ATT_TILE - counted_pos(p, 32 * wave), ATT_TILE, 32, p.radius);
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb) {
     s[kb] = dp[kb] = v16f{};

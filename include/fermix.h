@@ -500,7 +500,7 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * with causal, j <= offset + i. What is masked by lengths or mask may hold anything; a
  * value that causal alone masks has to be finite. Queries i >= q_lengths[b] (NULL: nq) get 0
  * and no gradient. Positions: q_pos (batch, nq), k_pos (batch, nk) together, or NULL: offset + i
- * and j. table (buckets, heads) float32 or NULL (no bias), map and radius as above, buckets <= FX_MAX_ATTENTION_BUCKETS;
+ * and j; 0 <= offset <= 2^31 - 1 - max(nq, nk). table (buckets, heads) float32 or NULL (no bias), map and radius as above, buckets <= FX_MAX_ATTENTION_BUCKETS;
  * its entries may be -inf, and entries of float32's lowest value weigh like any other.
  *
  * fx_attention_forward: out and, if given, stats (batch, heads, nq, 2): the largest S / scale and log2

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import fermix_amd as fx
-from tests.test_gpu_network import GATES, TYPES, ids
+from tests.test_gpu_network import GATES, TYPES, attention_case, check_attention, ids
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,18 @@ def test_norm_gate_without_rows(dev, dtype, gate, shape):
     del fill
     dg, dw = torch.autograd.grad((y, z), (g, w), (torch.zeros_like(y), torch.zeros_like(z)))
     assert dg.shape == g.shape and (dg == 0).all() and (dw == 0).all()
+
+
+# ------------------------------------------------------------------ the largest offsets
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("N,K,D,causal", [(65, 65, 16, False), (300, 200, 64, False), (200, 330, 128, False), (130, 130, 40, True), (100, 90, 64, True)],
+                         ids=lambda x: str(x))
+def test_attention_largest_offset(dev, dtype, N, K, D, causal):
+    """The last offset that is taken: every key is further below every query than the radius, also for tiles
+    whose distances reach the lowest int32, and nothing is hidden by causal."""
+    gen = torch.Generator().manual_seed(N + K)
+    c = attention_case(gen, dtype, 2, N, K, 2, 1, D)
+    c.update(causal=causal, offset=2**31 - 1 - max(N, K))
+    check_attention(c, dev, dtype, gen, (N, K, D, causal))

@@ -1,0 +1,35 @@
+"""The largest and smallest arguments that the network operators' C entry points and Python functions take, and what lies
+past them; before any device work (fake pointers, host only)."""
+
+import ctypes
+
+import pytest
+import torch
+
+import fermix_amd as fx
+from fermix_amd import _lib
+
+OK, INVALID, WORKSPACE, UNSUPPORTED = 0, 1, 2, 4
+GOOD = 0x10000
+
+
+def attention(**change):
+    a = _lib.FxAttention(batch=2, nq=5, nk=7, heads=4, kv_heads=2, dim=8, dtype=_lib.FX_BF16, scale=0.3, q=GOOD, k=GOOD, v=GOOD, out=GOOD)
+    for n, x in change.items():
+        setattr(a, n, x)
+    return ctypes.byref(a)
+
+
+def test_attention_offset():
+    """Positions offset + i stay within int32. (With no sample nothing is launched.)"""
+    L = _lib.lib()
+    last = 2**31 - 1 - 7
+    assert L.fx_attention_forward(attention(offset=last, batch=0), None) == OK
+    for bad in (last + 1, 2**31 - 1):
+        assert L.fx_attention_forward(attention(offset=bad, batch=0), None) == INVALID
+        assert L.fx_attention_grad(attention(offset=bad, batch=0), None, 0, None) == INVALID
+    x, k = torch.zeros(2, 5, 4, 8), torch.zeros(2, 7, 2, 8)
+    with pytest.raises(fx.FermixDeviceError):
+        fx.attention(x, k, k, offset=last)
+    with pytest.raises(ValueError):
+        fx.attention(x, k, k, offset=last + 1)
