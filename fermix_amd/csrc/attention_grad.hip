@@ -99,6 +99,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
   v16f dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = v16f{};
+  float fit = IS_F16<T> ? SCALE_START : 1.0f;
   TileLoad<T, DP, NT> kl, vl;
   KeyOf key{};  // of wave 0's lanes (GEN)
   auto fetch = [&](int k0) {
@@ -153,10 +154,14 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
         for (int i = 0; i < 16; ++i) sums.all += dp[i];
       }
       if (p.grad_table) bucket_add<GEN>(bv, kv, sums, dp, s, kb, k0, qpos, half, far, weights_on);
+      if constexpr (IS_F16<T>) {
+        fit_scale(fit, dp, dq);
+        dp *= fit;
+      }
       column_product<T, DP>(kt, 32 * kb, dp, dq, lane, p.dim);
     }
   }
-  store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale, p.dim, a.whole, half);
+  store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, p.scale / fit, p.dim, a.whole, half);
   // what dS add up to is delta's error: the second launch gets delta without it
   const float all = sizeof(T) == 2 || weights_on ? half_sum(sums.all) : 0.0f;
   if (qi < p.nq && half == 0) a.delta[stat] = delta + all;
@@ -257,6 +262,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
     sum[0][d] = v16f{};
     if (!SPLIT) sum[SPLIT ? 0 : 1][d] = v16f{};
   }
+  float fit = IS_F16<T> ? SCALE_START : 1.0f;  // of 2^WEIGHT_SHIFT dS
   // queries that some key of the workgroup is seen by
   const int first = p.causal ? max(0, k0 - p.offset) / ATT_TILE * ATT_TILE : 0;
   const int queries = k0 < klen ? qlen : 0;
@@ -294,7 +300,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
       if (threadIdx.x < ATT_TILE) {
         const bool exact = sizeof(T) == 4 || __any(fabsf(ml.x * a.c) > BASE_MAX);
         qv.max[threadIdx.x] = ml.x;
-        qv.log[threadIdx.x] = exact ? ml.y : ml.x * a.c + ml.y;
+        qv.log[threadIdx.x] = (exact ? ml.y : ml.x * a.c + ml.y) - WEIGHT_SHIFT<T>;
         if (threadIdx.x == 0) *qv.exact = exact;
         qv.delta[threadIdx.x] = de;
         if (GEN) qv.pos[threadIdx.x] = qp;
@@ -343,13 +349,19 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[4 * g + r] *= dp[4 * g + r] - de[r];
         }
+        if constexpr (IS_F16<T>) {
+          fit_scale(fit, s, sum[0]);
+          s *= fit;
+        }
         column_product<T, DP>(qt, 32 * qb, s, sum[0], lane, p.dim);
       }
     }
   }
   const int64_t row = ((at.b * p.nk + ki) * p.kv_heads + at.h) * p.dim;
-  if (do_k) store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, sum[0], p.scale, p.dim, a.whole, half);
-  if (do_v) store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, sum[SPLIT ? 0 : 1], 1.0f, p.dim, a.whole, half);
+  if (do_k)
+    store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, sum[0], p.scale * WEIGHT_UNIT<T> / fit, p.dim, a.whole, half);
+  if (do_v)
+    store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, sum[SPLIT ? 0 : 1], WEIGHT_UNIT<T>, p.dim, a.whole, half);
 }
 
 // Whether P is summed beside dS. For float32, whose delta is off by float32's roundings only, where these add up over many

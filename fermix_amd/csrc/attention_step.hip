@@ -489,7 +489,9 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float x = __builtin_amdgcn_exp2f(s[t][r] - ref);
+        float d = s[t][r] - ref;
+        if constexpr (IS_F16<T>) d += WEIGHT_SHIFT<T>;  // leaves the result, and the sums it is joined with, by l
+        const float x = __builtin_amdgcn_exp2f(d);
         sum += x;
         w[4 * t + r] = (T)x;
       }

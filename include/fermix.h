@@ -495,7 +495,8 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * q, out: (batch, nq, heads, dim), k, v: (batch, nk, kv_heads, dim), heads a multiple of kv_heads
  * (head h reads kv head h / (heads / kv_heads)), 1 <= dim <= 128, dtype FX_F32, FX_BF16 or
  * FX_F16; own strides in elements for batch, token and head, dim contiguous. Scores, softmax
- * and sums are float32; for the 16-bit types P (and dS) are rounded to dtype for the products.
+ * and sums are float32; for the 16-bit types P (and dS) are rounded to dtype for the products (float16: brought up by
+ * powers of two before, so that small weights and cotangents keep their digits).
  * Keys: index j < lengths[b] (NULL: nk), mask[b][j] != 0 (NULL: all; mask (batch, nk) bytes) and,
  * with causal, j <= offset + i. What is masked by lengths or mask may hold anything; a
  * value that causal alone masks has to be finite. Queries i >= q_lengths[b] (NULL: nq) get 0

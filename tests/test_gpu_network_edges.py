@@ -10,7 +10,7 @@ import torch
 
 import fermix_amd as fx
 from tests import network64 as ref
-from tests.test_gpu_network import GATES, TYPES, U, attention_case, check_attention, check_norm, ids, near_sums, norm_case, rand
+from tests.test_gpu_network import EPS, GATES, TYPES, U, attention_case, check_attention, check_norm, ids, near, near_sums, norm_case, rand, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -50,6 +50,64 @@ def test_attention_largest_offset(dev, dtype, N, K, D, causal):
     c = attention_case(gen, dtype, 2, N, K, 2, 1, D)
     c.update(causal=causal, offset=2**31 - 1 - max(N, K))
     check_attention(c, dev, dtype, gen, (N, K, D, causal))
+
+
+# ------------------------------------------------------------------ float16's small numbers
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4, "mixed"])
+@pytest.mark.parametrize("N,K,H,Hkv,D,mode", [(64, 4096, 2, 1, 64, ""), (4096, 64, 1, 1, 64, ""), (70, 2100, 2, 2, 128, "p"), (1100, 1100, 2, 1, 128, "c"),
+                                              (128, 128, 2, 2, 64, ""), (100, 128, 4, 2, 40, "lp"), (128, 90, 1, 1, 128, "m")], ids=lambda x: str(x))
+def test_attention_small_cotangents(dev, dtype, size, N, K, H, Hkv, D, mode):
+    """A loss that is a mean over many samples has small cotangents. P and dS then pass below float16's normal numbers
+    (dS below its smallest) where the gradients do not: the error stays that of the roundings. k is large for dq, then
+    q for dk, so that the results themselves are normal; "mixed": a cotangent of its own size for each query."""
+    gen = torch.Generator().manual_seed(N + K + D)
+    for big in "qk":
+        c = attention_case(gen, dtype, 1, N, K, H, Hkv, D, mode=mode)
+        small = "k" if big == "q" else "q"
+        c[big], c[small] = c[big] * 64, c[small] / 64
+        g = rand(gen, 1, N, H, D)
+        g = (g * (2.0 ** -torch.randint(0, 14, (1, N, 1, 1), generator=gen) if size == "mixed" else size)).to(dtype)
+        want = ref.attention(**c, grad=g)
+        got = run_attention(c, dev, g)
+        for name, x, y in zip(("out", "dq", "dk", "dv"), got, want):
+            near(x, y, dtype, 2, (big, name))
+        near_sums(got[4], want[4], want[5] + 1e-3 * want[5].mean(), dtype, what=(big, "dtable"), tol=EPS)
+
+
+@pytest.mark.parametrize("N,K,D", [(100, 128, 64), (90, 700, 40), (200, 300, 128)])
+def test_attention_large_cotangents(dev, N, K, D):
+    """dS past float16's largest number, where the gradients are within it (small q and k)."""
+    gen = torch.Generator().manual_seed(N)
+    c = attention_case(gen, torch.float16, 2, N, K, 2, 2, D)
+    c["q"], c["k"], c["v"] = c["q"] / 64, c["k"] / 64, c["v"] * 256
+    g = rand(gen, 2, N, 2, D, dtype=torch.float16, scale=100.0)
+    g[:, ::3] *= 100
+    want = ref.attention(**c, grad=g)
+    assert want[1].abs().max() < 6e4 and want[2].abs().max() < 6e4 and want[3].abs().max() < 6e4
+    got = run_attention(c, dev, g)
+    for name, x, y in zip(("out", "dq", "dk", "dv"), got, want):
+        near(x, y, torch.float16, 2, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("gap", [14.0, 16.0, 18.0])
+def test_attention_many_small_weights(dev, dtype, gap):
+    """One key outweighs each of the others by exp(gap), but its value is 0: what is left is the others' sum, whose
+    weights are below float16's normal numbers when the largest is 1. In a whole sequence and in one step."""
+    K, H, D = 3000, 4, 32
+    gen = torch.Generator().manual_seed(int(gap))
+    q = torch.full((1, 1, H, D), 1.0, dtype=dtype)
+    k, v = torch.zeros(1, K, 1, D, dtype=dtype), (1 + rand(gen, 1, K, 1, D, scale=0.25)).to(dtype)
+    k[0, 1234], v[0, 1234] = gap / D, 0.0
+    want = ref.attention(q, k, v, scale=1.0)
+    near(fx.attention(q.to(dev), k.to(dev), v.to(dev), scale=1.0), want, dtype, 2, "attention")
+    pages = torch.arange(K // 8, dtype=torch.int32, device=dev)[None]
+    kc, vc = (t.reshape(K // 8, 8, 1, D).to(dev) for t in (k, v))
+    got = fx.attention_step(q[:, 0].to(dev), kc, vc, pages, torch.tensor([K], dtype=torch.int32, device=dev), scale=1.0)
+    near(got, want[:, 0], dtype, 2, "step")
 
 
 # ------------------------------------------------------------------ more than one turn
