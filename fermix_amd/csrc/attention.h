@@ -385,20 +385,32 @@ struct AttArgs {
   float inv_scale;
   int weights;  // gradient: whether P is summed beside dS
   int tiles;   // items of a head
-  int64_t items;
+  int64_t first, items;  // of a launch
   float* delta;  // gradient: [batch][heads][nq] sum_d out grad_out
   float* part;   // gradient: bucket sums [head][batch * tiles][buckets]
 };
+
+// Launches for all items, each of at most as many as its lanes are counted in 32 bits. f(a) launches a.items workgroups.
+template <class F>
+void launch_items(const AttArgs& args, int tiles, int64_t items, int threads, F&& f) {
+  AttArgs a = args;
+  a.tiles = tiles;
+  const int64_t most = 0xffffffffll / threads;
+  for (a.first = 0; a.first < items; a.first += most) {
+    a.items = items - a.first < most ? items - a.first : most;
+    f(a);
+  }
+}
 
 // An item's place: sample, head and tile. The heads that share K and V follow each other; within a head the tile with
 // the most work under causal comes first: the last of the queries (last_first), the first of the keys.
 struct Place {
   int64_t b;
   int h, tile;
-  __device__ __forceinline__ Place(int64_t item, int heads, int tiles, bool last_first) {
-    const int64_t bh = item / tiles;
-    tile = (int)(item - bh * tiles);
-    if (last_first) tile = tiles - 1 - tile;
+  __device__ __forceinline__ Place(const AttArgs& a, int heads, bool last_first) {
+    const int64_t item = a.first + xcd_item(blockIdx.x, a.items), bh = item / a.tiles;
+    tile = (int)(item - bh * a.tiles);
+    if (last_first) tile = a.tiles - 1 - tile;
     b = bh / heads;
     h = (int)(bh - b * heads);
   }

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
   if (GEN) rest += 272;
   const BiasView bv(GEN, rest, p.radius);
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles, true);
+  const Place at(a, p.heads, true);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int q0 = at.tile * 32 * WAVES, qi = q0 + 32 * wave + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
       store_low<T, DP>(static_cast<_Float16*>(p.out_low) + row * p.dim, out_in, o, inv, p.dim, a.whole, half);
   if (p.stats && out_in && half == 0)
     reinterpret_cast<float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi] =
-        l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l) - WEIGHT_SHIFT<T>);
+        l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l * WEIGHT_UNIT<T>));
 }
 
 int forward_waves(const fx_attention& p) { return p.dim > 64 && p.dtype != FX_F32 && p.nq > 128 ? 8 : 4; }
@@ -195,11 +195,8 @@ extern "C" int fx_attention_forward(const fx_attention* p, fx_stream_t stream) {
   if (!attention_sizes_ok(p)) return FX_ERR_INVALID_ARGUMENT;
   if (p->batch == 0 || p->nq == 0) return FX_OK;
   if (!attention_pointers_ok(*p)) return FX_ERR_INVALID_ARGUMENT;
-  AttArgs a = attention_args(*p);
-  const int waves = forward_waves(*p);
-  a.tiles = (int)cdiv(p->nq, 32 * waves);
-  a.items = p->batch * p->heads * a.tiles;
-  if (a.items > 0x7fffffff) return FX_ERR_UNSUPPORTED;
+  const AttArgs args = attention_args(*p);
+  const int waves = forward_waves(*p), tiles = (int)cdiv(p->nq, 32 * waves);
   return attention_shape(*p, [&](auto t, auto dp, auto gen) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
@@ -207,8 +204,10 @@ extern "C" int fx_attention_forward(const fx_attention* p, fx_stream_t stream) {
     const size_t lds = forward_lds<T, DP>(GEN, p->radius);
     auto go = [&](auto w) {
       constexpr int WAVES = decltype(w)::value;
-      hipLaunchKernelGGL((attention_kernel<T, DP, GEN, WAVES>), dim3((unsigned)a.items), dim3(64 * WAVES), lds,
-                         (hipStream_t)stream, a);
+      launch_items(args, tiles, p->batch * p->heads * tiles, 64 * WAVES, [&](const AttArgs& a) {
+        hipLaunchKernelGGL((attention_kernel<T, DP, GEN, WAVES>), dim3((unsigned)a.items), dim3(64 * WAVES), lds,
+                           (hipStream_t)stream, a);
+      });
     };
     if constexpr (DP == 128 && sizeof(T) == 2)
       if (waves == 8) return go(ic<8>{});

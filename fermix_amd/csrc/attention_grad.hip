@@ -47,7 +47,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 && !(DP == 1
   float* const ds_sums = row_sum + 32 * WAVES;                                             // [wave][bucket][64]
   unsigned* const weights = reinterpret_cast<unsigned*>(ds_sums + 64 * WAVES * p.buckets);  // [wave][bucket][32]
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.heads, a.tiles, true);
+  const Place at(a, p.heads, true);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int q0 = at.tile * 32 * WAVES, qi = q0 + 32 * wave + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
   rest += 1040;
   const BiasView bv(GEN, rest, p.radius);
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.kv_heads, a.tiles, false);  // heads: those of k and v
+  const Place at(a, p.kv_heads, false);  // heads: those of k and v
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, half = lane >> 5;
   const bool do_v = !SPLIT || threadIdx.x < 256, do_k = !SPLIT || threadIdx.x >= 256;
   const int k0 = at.tile * 128, kw = k0 + 32 * wave, ki = kw + (lane & 31);
@@ -412,21 +412,16 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
       return FX_ERR_WORKSPACE;
   }
   if (p->nk > 0 && (!p->k || !p->v || !p->grad_k || !p->grad_v)) return FX_ERR_INVALID_ARGUMENT;
-  AttArgs a = attention_args(*p);
-  a.delta = static_cast<float*>(workspace);
-  a.part = a.delta + delta_floats(*p);
-  a.weights = sums_weights(*p);
+  AttArgs args = attention_args(*p);
+  args.delta = static_cast<float*>(workspace);
+  args.part = args.delta + delta_floats(*p);
+  args.weights = sums_weights(*p);
   const bool in_short = attention_grad_short_fits(*p), own = p->heads == p->kv_heads;
   if (in_short) {
-    a.tiles = 1;
-    a.items = p->batch * p->heads;
-    if (a.items > 0x7fffffff) return FX_ERR_UNSUPPORTED;
-    const int st = launch_attention_grad_short(a, s);
+    const int st = launch_attention_grad_short(args, s);
     if (st != FX_OK) return st;
   }
   const int waves = dq_waves(*p), qtiles = (int)cdiv(p->nq, 32 * waves), ktiles = (int)cdiv(p->nk, 128);
-  if (p->batch * p->heads * qtiles > 0x7fffffff || p->batch * p->kv_heads * ktiles > 0x7fffffff)
-    return FX_ERR_UNSUPPORTED;
   const int st = attention_shape(*p, [&](auto t, auto dp, auto gen) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
@@ -436,12 +431,12 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
     const size_t lds_kv = tiles + 1040 + view;
     constexpr bool LONG_ROWS = DP == 128 && sizeof(T) == 2;
     if (qtiles && !in_short) {
-      a.tiles = qtiles;
-      a.items = p->batch * p->heads * qtiles;
       auto go = [&](auto w) {
         constexpr int WAVES = decltype(w)::value;
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP, GEN, WAVES>), dim3((unsigned)a.items), dim3(64 * WAVES), lds_q, s,
-                           a);
+        launch_items(args, qtiles, p->batch * p->heads * qtiles, 64 * WAVES, [&](const AttArgs& a) {
+          hipLaunchKernelGGL((attention_dq_kernel<T, DP, GEN, WAVES>), dim3((unsigned)a.items), dim3(64 * WAVES), lds_q,
+                             s, a);
+        });
       };
       if constexpr (LONG_ROWS) {
         if (waves == 8)
@@ -453,14 +448,15 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
       }
     }
     if (ktiles && !(in_short && own)) {
-      a.tiles = ktiles;
-      a.items = p->batch * p->kv_heads * ktiles;
-      hipLaunchKernelGGL((attention_dkv_kernel<T, DP, GEN, LONG_ROWS>), dim3((unsigned)a.items),
-                         dim3(LONG_ROWS ? 512 : 256), lds_kv, s, a);
+      constexpr int NT = LONG_ROWS ? 512 : 256;
+      launch_items(args, ktiles, p->batch * p->kv_heads * ktiles, NT, [&](const AttArgs& a) {
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, GEN, LONG_ROWS>), dim3((unsigned)a.items), dim3(NT), lds_kv, s,
+                           a);
+      });
     }
   });
   if (st != FX_OK || !p->grad_table) return st;
-  return launch_bucket_join(a.part, p->batch * qtiles, p->buckets, p->heads, p->grad_table, s);
+  return launch_bucket_join(args.part, p->batch * qtiles, p->buckets, p->heads, p->grad_table, s);
 }
 
 }  // extern "C"

@@ -47,7 +47,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
   float* const ds_sums = reinterpret_cast<float*>(rest);  // [wave][bucket][64]
   T* const ps = reinterpret_cast<T*>(rest);               // then [query][key]
 
-  const Place at(xcd_item(blockIdx.x, a.items), p.heads, 1, true);
+  const Place at(a, p.heads, true);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int qi = 32 * wave + (lane & 31);
   const int qlen = p.q_lengths ? max(0, min(p.q_lengths[at.b], p.nq)) : p.nq;
@@ -241,19 +241,21 @@ bool attention_grad_short_fits(const fx_attention& p) {
   return p.dtype != FX_F32 && p.nq >= 1 && p.nq <= SHORT && p.nk >= 1 && p.nk <= SHORT;
 }
 
-int launch_attention_grad_short(const AttArgs& a, hipStream_t s) {
-  const fx_attention& p = a.p;
+int launch_attention_grad_short(const AttArgs& args, hipStream_t s) {
+  const fx_attention& p = args.p;
   auto go = [&](auto t, auto dp, auto gen) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool GEN = decltype(gen)::value != 0;
     const bool own = p.heads == p.kv_heads;
     const size_t lds = short_lds<T, DP>(view_lds(GEN, p.radius), p.buckets, p.grad_table != nullptr, own);
-    const dim3 grid((unsigned)a.items), block(SHORT_NT);
-    if (own)
-      hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN, true>), grid, block, lds, s, a);
-    else
-      hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN, false>), grid, block, lds, s, a);
+    launch_items(args, 1, p.batch * p.heads, SHORT_NT, [&](const AttArgs& a) {
+      const dim3 grid((unsigned)a.items), block(SHORT_NT);
+      if (own)
+        hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN, true>), grid, block, lds, s, a);
+      else
+        hipLaunchKernelGGL((attention_short_grad_kernel<T, DP, GEN, false>), grid, block, lds, s, a);
+    });
   };
   return attention_shape(p, [&](auto t, auto dp, auto gen) {
     if constexpr (sizeof(t) == 2) go(t, dp, gen);

@@ -429,28 +429,30 @@ __global__ __launch_bounds__(JOIN_NT) void columns_join_kernel(const JoinArgs a)
 
 // The gate's gradient of each sample from its items' column sums: per column, or (gc == 0) over them. Zero without
 // items (no rows).
+constexpr int64_t GATE_GROUPS = 1 << 20;  // most workgroups for the samples (a launch's lanes are counted in 32 bits)
 template <class T>
 __global__ __launch_bounds__(256) void gate_join_kernel(const float* part, int64_t samples, int64_t chunks, int C,
                                                         int gc, T* out) {
-  const int64_t sample = blockIdx.x;
-  const float* p = part + sample * chunks * C;
-  if (gc) {
-    for (int c = blockIdx.y * 256 + threadIdx.x; c < C; c += 256 * gridDim.y) {
+  __shared__ double s[256];
+  for (int64_t sample = blockIdx.x; sample < samples; sample += gridDim.x) {
+    const float* p = part + sample * chunks * C;
+    if (gc) {
+      for (int c = blockIdx.y * 256 + threadIdx.x; c < C; c += 256 * gridDim.y) {
+        double x = 0.0;
+        for (int64_t i = 0; i < chunks; ++i) x += (double)p[i * C + c];
+        out[sample * C + c] = (T)x;
+      }
+    } else {
       double x = 0.0;
-      for (int64_t i = 0; i < chunks; ++i) x += (double)p[i * C + c];
-      out[sample * C + c] = (T)x;
-    }
-  } else {
-    __shared__ double s[256];
-    double x = 0.0;
-    for (int64_t i = threadIdx.x; i < chunks * C; i += 256) x += (double)p[i];
-    s[threadIdx.x] = x;
-    __syncthreads();
-    for (int m = 128; m; m >>= 1) {
-      if ((int)threadIdx.x < m) s[threadIdx.x] += s[threadIdx.x + m];
+      for (int64_t i = threadIdx.x; i < chunks * C; i += 256) x += (double)p[i];
+      s[threadIdx.x] = x;
       __syncthreads();
+      for (int m = 128; m; m >>= 1) {
+        if ((int)threadIdx.x < m) s[threadIdx.x] += s[threadIdx.x + m];
+        __syncthreads();
+      }
+      if (threadIdx.x == 0) out[sample] = (T)s[0];
     }
-    if (threadIdx.x == 0) out[sample] = (T)s[0];
   }
 }
 
@@ -601,9 +603,11 @@ int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t wor
                {p->grad_post_weight, p->grad_post_bias, p->grad_scale, p->grad_pre_weight, p->grad_pre_bias}};
     hipLaunchKernelGGL((columns_join_kernel<T>), dim3((p->columns + JOIN_COLUMNS - 1) / JOIN_COLUMNS, Q_COLUMNS),
                        dim3(JOIN_NT), 0, s, j);
-    if (gates)
-      hipLaunchKernelGGL((gate_join_kernel<T>), dim3((unsigned)gates, p->gc ? (p->columns + 255) / 256 : 1), dim3(256),
-                         0, s, a.gate_part, gates, n.chunks, p->columns, (int)p->gc, static_cast<T*>(p->grad_gate));
+    if (gates) {
+      const dim3 grid((unsigned)(gates < GATE_GROUPS ? gates : GATE_GROUPS), p->gc ? (p->columns + 255) / 256 : 1);
+      hipLaunchKernelGGL((gate_join_kernel<T>), grid, dim3(256), 0, s, a.gate_part, gates, n.chunks, p->columns,
+                         (int)p->gc, static_cast<T*>(p->grad_gate));
+    }
     return launched();
   });
 }

@@ -155,3 +155,41 @@ def test_relative_bias_gradient_of_one_workgroup(dev):
         (dt,) = torch.autograd.grad(fx.relative_bias(t, m.to(dev), p.to(dev), p.to(dev)), t, g.to(dev))
         want = ref.bucket_sums(g.double(), ref.bucket_of(m, 32, p, p), 32)
         near_sums(dt, want, want, torch.float32, tol=2 * U[torch.float32])
+
+
+# ------------------------------------------------------------------ more than one launch
+
+
+MANY = 2**32 // 256 + 12345  # workgroups of 256 lanes, which a launch counts in 32 bits
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("Hkv", [2, 1])
+def test_attention_many_items(dev, dtype, Hkv):
+    """One query, one key: out is v, dv the cotangent (summed over heads that share it), the other gradients vanish: the
+    16-bit types form P = 1 from a score that has been rounded, to EPS, and so dS = P (dP - P dP) to EPS of dP."""
+    gen = torch.Generator(device=dev).manual_seed(1)
+    B = MANY // Hkv + 1
+    r = lambda H: torch.randn(B, 1, H, 1, generator=gen, device=dev).to(dtype)
+    q, k, v, g = r(2), r(Hkv), r(Hkv), r(2)
+    table = torch.zeros(2, 2, device=dev)
+    leaves = [x.requires_grad_(True) for x in (q, k, v, table)]
+    out = fx.attention(q, k, v, table=table, buckets=torch.zeros(1, dtype=torch.uint8, device=dev))
+    assert torch.equal(out, v.detach().expand(B, 1, 2, 1))
+    dq, dk, dv, dt = torch.autograd.grad(out, leaves, g)
+    dp = (g * v).detach().abs().double()
+    tol = 0.0 if dtype == torch.float32 else EPS
+    assert (dq.double().abs() <= tol * dp * k.detach().abs()).all() and dt.abs().max() <= tol * dp.sum()
+    assert (dk.double().abs() <= tol * (dp * q.detach().abs()).reshape(B, 1, Hkv, -1).sum(-1, keepdim=True)).all()
+    assert torch.equal(dv, g if Hkv == 2 else (g[:, :, :1].float() + g[:, :, 1:].float()).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_norm_gate_of_many_samples(dev, dtype):
+    gen = torch.Generator(device=dev).manual_seed(2)
+    x, h, g, dy = (torch.randn(MANY, 1, 1, generator=gen, device=dev).to(dtype) for _ in range(4))
+    for t in (h, g):
+        t.requires_grad_(True)
+    y = fx.residual_norm(x, h, gate=g, post_norm=False, pre_norm=False)
+    dh, dg = torch.autograd.grad(y, (h, g), dy)
+    assert torch.equal(dh, dy * g) and torch.equal(dg, dy * h)
