@@ -157,11 +157,11 @@ __global__ __launch_bounds__(64 * W) void bias_grad_kernel(const BiasArgs a) {
   __syncthreads();
   A* out = static_cast<A*>(a.out) + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.buckets;
   for (int t = threadIdx.x; t < a.buckets; t += 64 * W) {
-    double s = 0.0;
+    double s[4] = {};  // four chains, so that an add does not wait for the one before it
     for (int w = 0; w < W; ++w)
 #pragma unroll 4
-      for (int l = 0; l < 64; ++l) s += (double)sums[(w * a.buckets + t) * 64 + ((l + t) & 63)];  // rotated: no shared bank
-    out[t] = (A)s;
+      for (int l = 0; l < 64; ++l) s[l & 3] += (double)sums[(w * a.buckets + t) * 64 + ((l + t) & 63)];  // rotated: no shared bank
+    out[t] = (A)((s[0] + s[1]) + (s[2] + s[3]));
   }
 }
 
