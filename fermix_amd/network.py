@@ -19,6 +19,7 @@ import ctypes
 import math
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -77,9 +78,16 @@ def _wants_grad(*xs):
     return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)
 
 
+def _through_autograd(*xs):
+    """Whether a call goes through its autograd function: where a gradient is wanted, and under torch.jit.trace, which
+    records that and would otherwise record the allocation of the results alone."""
+    return _wants_grad(*xs) or torch.jit.is_tracing()
+
+
 def _refuse_forward_mode(*xs):
-    """A dual tensor that needs no gradient would go to the kernels as its primal and come back without a tangent."""
-    if any(x is not None and _dual(x) for x in xs):
+    """A dual tensor that needs no gradient would go to the kernels as its primal and come back without a tangent. (There
+    are none outside a level of forward mode: looking at each tensor then is 1 us of every call.)"""
+    if fwAD._current_level >= 0 and any(x is not None and _dual(x) for x in xs):
         raise NotImplementedError("fermix_amd's network operators have no forward mode: differentiate them in reverse mode")
 
 
@@ -189,7 +197,7 @@ def relative_bias(table, buckets, q_pos, k_pos):
         lead = torch.broadcast_shapes(lead, k.shape[:-1])
         q, k = (x.expand(lead + x.shape[-1:]).reshape(math.prod(lead), x.shape[-1]) for x in (q, k))
     q, k = _int32(q), _int32(k)
-    if _wants_grad(table):
+    if _through_autograd(table):
         out = _RelativeBias.apply(table, buckets, q, k)
     else:
         out = _bias_forward(table.contiguous(), buckets, q, k)
@@ -325,7 +333,7 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     q_pos, k_pos, lengths, q_lengths = (None if x is None else _int32(x) for x in (q_pos, k_pos, lengths, q_lengths))
     mask = None if mask is None else mask.contiguous()
     rest = (buckets, q_pos, k_pos, lengths, q_lengths, mask, bool(causal), offset, scale)
-    if _wants_grad(q, k, v, table):
+    if _through_autograd(q, k, v, table):
         return _Attention.apply(q, k, v, table, *rest)
     out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
     _call("fx_attention_forward", q, ctypes.byref(_attention_args(q, k, v, table, *rest, out, None)))
@@ -371,6 +379,8 @@ def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table
     _on_device(q)
     if _wants_grad(q, k_cache, v_cache, k, v, table):
         raise NotImplementedError("attention_step has no gradient: call it under torch.no_grad(), or train with attention")
+    if torch.jit.is_tracing():
+        raise NotImplementedError("attention_step writes the caches in place, which torch.jit.trace does not record")
     q, pages, lengths = q.contiguous(), _int32(pages), _int32(lengths)
     k, v = (None if x is None else x.contiguous() for x in (k, v))
     out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
@@ -523,7 +533,7 @@ def residual_norm(x, h, *, post_weight=None, post_bias=None, gate=None, scale=No
     _on_device(x)
     flags = (FX_NORM_LAYER if norm == "layer" else 0) | (FX_NORM_POST if post_norm else 0) | (FX_NORM_PRE if pre_norm else 0)
     x, h = x.contiguous(), h.contiguous()
-    if _wants_grad(x, h, gate, *columns):
+    if _through_autograd(x, h, gate, *columns):
         return _ResidualNorm.apply(x, h, gate, *columns, alpha, float(eps), flags)
     y = torch.empty_like(x)
     z = torch.empty_like(x) if pre_norm else None

@@ -193,3 +193,28 @@ def test_norm_gate_of_many_samples(dev, dtype):
     y = fx.residual_norm(x, h, gate=g, post_norm=False, pre_norm=False)
     dh, dg = torch.autograd.grad(y, (h, g), dy)
     assert torch.equal(dh, dy * g) and torch.equal(dg, dy * h)
+
+
+# ------------------------------------------------------------------ tracing
+
+
+def test_traces_replay_on_other_inputs(dev):
+    """torch.jit.trace records a call, not only the memory that it returns: a replay gives the new input's values."""
+    p = torch.arange(12, dtype=torch.int32, device=dev)[None]
+    m, table = fx.distance_buckets(device=dev), torch.randn(32, 2, device=dev)
+    calls = {
+        (32, 2): lambda t: fx.relative_bias(t, m, p, p),
+        (2, 12, 2, 16): lambda x: fx.attention(x, x, x, table=table, buckets=m, causal=True),
+        (3, 5, 64): lambda x: fx.residual_norm(x, 2 * x, gate=x)[1],
+    }
+    for shape, f in calls.items():
+        traced = torch.jit.trace(f, (torch.randn(shape, device=dev),), check_trace=False)
+        for _ in range(3):
+            x = torch.randn(shape, device=dev)
+            fill = [torch.full((n,), math.nan, device=dev) for n in (256, 768, 960, 2048) for _ in range(8)]
+            del fill
+            assert torch.equal(traced(x), f(x)), shape
+    cache = torch.zeros(3, 4, 2, 16, device=dev)
+    z = torch.zeros(2, 1, dtype=torch.int32, device=dev)
+    with pytest.raises(NotImplementedError, match="trace"):
+        torch.jit.trace(lambda q: fx.attention_step(q, cache, cache.clone(), z, z[:, 0]), (torch.randn(2, 4, 16, device=dev),))
