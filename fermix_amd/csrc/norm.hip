@@ -427,8 +427,8 @@ __global__ __launch_bounds__(JOIN_NT) void columns_join_kernel(const JoinArgs a)
   }
 }
 
-// The gate's gradient of each sample from its items' column sums: per column, or (gc == 0) over them. Zero without
-// items (no rows).
+// The gate's gradient of each sample (or of all: one) from its items' column sums: per column, or (gc == 0) over
+// them. Zero without items (no rows).
 constexpr int64_t GATE_GROUPS = 1 << 20;  // most workgroups for the samples (a launch's lanes are counted in 32 bits)
 template <class T>
 __global__ __launch_bounds__(256) void gate_join_kernel(const float* part, int64_t samples, int64_t chunks, int C,
@@ -567,10 +567,11 @@ size_t fx_residual_norm_grad_workspace(const fx_residual_norm* p) {
 
 int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t workspace_bytes, fx_stream_t stream) {
   if (!norm_sizes_ok(p)) return FX_ERR_INVALID_ARGUMENT;
+  if (p->gate && p->gr && !p->gs && p->samples > 1) return FX_ERR_UNSUPPORTED;  // sums over samples, not rows
   const hipStream_t s = (hipStream_t)stream;
   const bool none = p->samples == 0 || p->rows == 0;
   // values (or rows of columns) of a gate that is summed over the rows: there are some even where there are no rows
-  const int64_t gates = !p->gate || p->gr ? 0 : none && !p->gs ? 1 : p->samples;
+  const int64_t gates = !p->gate || p->gr ? 0 : p->gs ? p->samples : 1;
   if (gates && (!p->grad_gate || !aligned(p->grad_gate, dtype_size(p->dtype)))) return FX_ERR_INVALID_ARGUMENT;
   if (!none) {
     if (!norm_pointers_ok(*p) || !p->stats || (p->gate && !p->grad_gate)) return FX_ERR_INVALID_ARGUMENT;
@@ -605,7 +606,7 @@ int fx_residual_norm_grad(const fx_residual_norm* p, void* workspace, size_t wor
                        dim3(JOIN_NT), 0, s, j);
     if (gates) {
       const dim3 grid((unsigned)(gates < GATE_GROUPS ? gates : GATE_GROUPS), p->gc ? (p->columns + 255) / 256 : 1);
-      hipLaunchKernelGGL((gate_join_kernel<T>), grid, dim3(256), 0, s, a.gate_part, gates, n.chunks, p->columns,
+      hipLaunchKernelGGL((gate_join_kernel<T>), grid, dim3(256), 0, s, a.gate_part, gates, n.items / gates, p->columns,
                          (int)p->gc, static_cast<T*>(p->grad_gate));
     }
     return launched();

@@ -591,7 +591,8 @@ typedef struct fx_residual_norm {
   void *y, *z; /* forward */
   float* stats;
   /* gradient: cotangents (either may be NULL: zero) and results; grad_gate (a gate given) has
-   * the gate's broadcast shape: samples x rows x columns, 1 wherever its stride is zero, packed.
+   * the gate's broadcast shape: samples x rows x columns, 1 wherever its stride is zero, packed; a gate with
+   * strides over the rows alone has a gradient for one sample only (FX_ERR_UNSUPPORTED: swap samples and rows).
    * The five column gradients (columns, of wdtype) may each be NULL. */
   const void *grad_y, *grad_z;
   void *grad_x, *grad_h, *grad_gate;

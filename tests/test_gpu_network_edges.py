@@ -3,12 +3,14 @@ nothing to work on, the largest offsets, more work than one launch or one pass o
 holds, cotangents and weights that are small for float16. Oracle and tolerances: those of
 test_gpu_network.py, unless a test derives its own."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import fermix_amd as fx
+from fermix_amd import _lib, network
 from tests import network64 as ref
 from tests.test_gpu_network import EPS, GATES, TYPES, U, attention_case, check_attention, check_norm, ids, near, near_sums, norm_case, rand, run_attention
 
@@ -218,3 +220,33 @@ def test_traces_replay_on_other_inputs(dev):
     z = torch.zeros(2, 1, dtype=torch.int32, device=dev)
     with pytest.raises(NotImplementedError, match="trace"):
         torch.jit.trace(lambda q: fx.attention_step(q, cache, cache.clone(), z, z[:, 0]), (torch.randn(2, 4, 16, device=dev),))
+
+
+# ------------------------------------------------------------------ the C entry points' own layouts
+
+
+@pytest.mark.parametrize("gc", [1, 0])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_norm_gate_shared_by_samples(dev, dtype, gc):
+    """A gate with no stride over samples and rows has one gradient, of the shape that its strides name, and nothing is
+    written past it."""
+    gen = torch.Generator().manual_seed(3)
+    c = norm_case(gen, dtype, (7, 40, 96), "channel" if gc else "scalar", "")
+    grads = rand(gen, 7, 40, 96, dtype=dtype), rand(gen, 7, 40, 96, dtype=dtype)
+    want = ref.residual_norm(**c, grads=grads)[2]
+    a = {n: x.to(dev) for n, x in c.items()}
+    y, z, dx, dh = (torch.empty_like(a["x"]) for _ in range(4))
+    stats = torch.empty(7, 40, 4, device=dev)
+    s = network._norm_args(a["x"], a["h"], a["gate"], [None] * 5, 1.0, 1e-6, _lib.FX_NORM_POST | _lib.FX_NORM_PRE, y, z, stats)
+    s.samples, s.rows, s.xs, s.hs, s.os = 7, 40, 40 * 96, 40 * 96, 40 * 96
+    assert (s.gs, s.gr, s.gc) == (0, 0, gc)
+    network._call("fx_residual_norm_forward", y, ctypes.byref(s))
+    dy, dz = (g.to(dev) for g in grads)
+    n = 96 if gc else 1
+    dg = torch.full((8 * n,), 7.0, dtype=dtype, device=dev)
+    s.grad_y, s.grad_z, s.grad_x, s.grad_h, s.grad_gate = (t.data_ptr() for t in (dy, dz, dx, dh, dg))
+    size = _lib.lib().fx_residual_norm_grad_workspace(ctypes.byref(s))
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    network._call("fx_residual_norm_grad", y, ctypes.byref(s), ws.data_ptr(), size)
+    near_sums(dg[:n].reshape(want["gate"].shape), want["gate"], want["size_gate"], dtype, dtype)
+    assert (dg[n:] == 7.0).all()

@@ -33,3 +33,15 @@ def test_attention_offset():
         fx.attention(x, k, k, offset=last)
     with pytest.raises(ValueError):
         fx.attention(x, k, k, offset=last + 1)
+
+
+def test_norm_gate_of_the_rows_alone():
+    """The gradient of a gate that samples share and rows do not is a sum over samples: refused before any work."""
+    L = _lib.lib()
+    a = _lib.FxResidualNorm(samples=2, rows=3, columns=8, dtype=_lib.FX_BF16, wdtype=_lib.FX_F32, flags=6, eps=1e-6, alpha=1.0, x=GOOD, h=GOOD,
+                            gate=GOOD, xs=24, xr=8, hs=24, hr=8, os=24, or_=8, gr=8, gc=1, stats=GOOD, grad_y=GOOD, grad_gate=GOOD)
+    assert L.fx_residual_norm_grad(ctypes.byref(a), None, 0, None) == UNSUPPORTED
+    a.gs = 24
+    assert L.fx_residual_norm_grad(ctypes.byref(a), None, 0, None) == WORKSPACE
+    a.gs, a.samples = 0, 1
+    assert L.fx_residual_norm_grad(ctypes.byref(a), None, 0, None) == WORKSPACE
