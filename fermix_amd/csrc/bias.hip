@@ -28,7 +28,11 @@ struct BiasArgs {
   int64_t batch;
   int heads, nq, nk;
   void* out;  // gradient: the workgroups' sums
+  int first, some;  // values: heads of this launch
 };
+
+// Bytes of the table that a workgroup of the values' launch holds; further heads take launches of their own.
+constexpr int64_t BIAS_TABLE = 64 * 1024;
 
 // How a workgroup of nt lanes goes over the pairs: 2^shift lanes take a row's vectors (of V keys) in turn, the rest
 // of it further rows; an item is BIAS_UNROLL x BIAS_TURNS such sets of rows of one sample. A lane's keys
@@ -75,17 +79,17 @@ template <class T, int V>
 __global__ __launch_bounds__(BIAS_NT) void bias_kernel(const BiasArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   T* tab = reinterpret_cast<T*>(smem);  // [head][bucket]
-  unsigned char* map = smem + (size_t)a.heads * a.buckets * sizeof(T);
-  const T* table = static_cast<const T*>(a.table);
-  for (int i = threadIdx.x; i < a.heads * a.buckets; i += BIAS_NT)
-    tab[i] = table[(i % a.buckets) * a.heads + i / a.buckets];
+  unsigned char* map = smem + (size_t)a.some * a.buckets * sizeof(T);
+  const T* table = static_cast<const T*>(a.table) + a.first;
+  for (int i = threadIdx.x; i < a.some * a.buckets; i += BIAS_NT)
+    tab[i] = table[(int64_t)(i % a.buckets) * a.heads + i / a.buckets];
   stage_map(a, map, BIAS_NT);
   __syncthreads();
   for_items<V>(a, BIAS_NT, [&](int64_t b, int first, int end, int step, int key) {
     int k[V];
     load_keys<V>(a.k_pos + b * a.nk + key, k);
     const int* qp = a.q_pos + b * a.nq;
-    T* const out = static_cast<T*>(a.out) + b * a.heads * a.nq * (int64_t)a.nk + key;
+    T* const out = static_cast<T*>(a.out) + (b * a.heads + a.first) * a.nq * (int64_t)a.nk + key;
 #pragma unroll 2
     for (int i = first; i < end; i += step) {
       const int q = qp[i];
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(BIAS_NT) void bias_kernel(const BiasArgs a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) bucket[v] = distance_bucket(map, a.radius, k[v], q);
       T* o = out + (int64_t)i * a.nk;
-      for (int h = 0; h < a.heads; ++h, o += (int64_t)a.nq * a.nk) {
+      for (int h = 0; h < a.some; ++h, o += (int64_t)a.nq * a.nk) {
         vec_t<T, V> x;
 #pragma unroll
         for (int v = 0; v < V; ++v) x[v] = tab[h * a.buckets + bucket[v]];
@@ -198,7 +202,8 @@ int bias_vec(int nk, size_t size, const void* p) {
 bool bias_sizes_ok(int32_t radius, int32_t buckets, int64_t batch, int32_t heads, int32_t nq, int32_t nk,
                    int32_t dtype) {
   return radius >= 0 && radius <= FX_MAX_RADIUS && buckets >= 1 && buckets <= 256 && batch >= 0 && heads >= 1 &&
-         heads <= 4096 && nq >= 0 && nk >= 0 && dtype_size(dtype);
+         heads <= FX_MAX_BIAS_HEADS && nq >= 0 && nq <= FX_MAX_POSITIONS && nk >= 0 && nk <= FX_MAX_POSITIONS &&
+         dtype_size(dtype);
 }
 
 }  // namespace
@@ -222,23 +227,26 @@ int fx_relative_bias(const void* table, const uint8_t* map, int32_t radius, int3
                      void* out, fx_stream_t stream) {
   if (!bias_sizes_ok(radius, buckets, batch, heads, nq, nk, dtype)) return FX_ERR_INVALID_ARGUMENT;
   const size_t size = dtype_size(dtype);
-  if ((size_t)heads * buckets * size > 64 * 1024) return FX_ERR_UNSUPPORTED;
   if (batch == 0 || nq == 0 || nk == 0) return FX_OK;
   if (!table || !map || !q_pos || !k_pos || !out || !aligned(table, size) || !aligned(out, size) ||
       !aligned(q_pos, 4) || !aligned(k_pos, 4))
     return FX_ERR_INVALID_ARGUMENT;
-  const BiasArgs a{table, map, radius, buckets, q_pos, k_pos, batch, heads, nq, nk, out};
+  BiasArgs a{table, map, radius, buckets, q_pos, k_pos, batch, heads, nq, nk, out};
+  const int at_once = (int)(BIAS_TABLE / (buckets * size));
   return with_type<true>(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int V = VEC16<T>;
     const int v = bias_vec(nk, sizeof(T), out);
     const int64_t most = Tiling(BIAS_NT, batch, nq, nk / v).items;
     const unsigned grid = (unsigned)(most < 4096 ? most : 4096);
-    const size_t lds = (size_t)heads * buckets * sizeof(T) + 2 * radius + 1;
-    if (v == V)
-      hipLaunchKernelGGL((bias_kernel<T, V>), dim3(grid), dim3(BIAS_NT), lds, (hipStream_t)stream, a);
-    else
-      hipLaunchKernelGGL((bias_kernel<T, 1>), dim3(grid), dim3(BIAS_NT), lds, (hipStream_t)stream, a);
+    for (a.first = 0; a.first < heads; a.first += at_once) {
+      a.some = heads - a.first < at_once ? heads - a.first : at_once;
+      const size_t lds = (size_t)a.some * buckets * sizeof(T) + 2 * radius + 1;
+      if (v == V)
+        hipLaunchKernelGGL((bias_kernel<T, V>), dim3(grid), dim3(BIAS_NT), lds, (hipStream_t)stream, a);
+      else
+        hipLaunchKernelGGL((bias_kernel<T, 1>), dim3(grid), dim3(BIAS_NT), lds, (hipStream_t)stream, a);
+    }
     return launched();
   });
 }
@@ -275,7 +283,7 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
     int64_t groups = 0;
     if (!none) {
       const int v = bias_vec(nk, sizeof(T), grad_out);
-      const BiasArgs a{grad_out, map, radius, buckets, q_pos, k_pos, batch, heads, nq, nk, workspace};
+      const BiasArgs a{grad_out, map, radius, buckets, q_pos, k_pos, batch, heads, nq, nk, workspace, 0, heads};
       const int w = bias_waves(buckets);
       groups = bias_grad_groups(buckets, batch, heads, nq, nk, v);
       const size_t lds = (size_t)w * buckets * 64 * sizeof(A) + 2 * radius + 1;

@@ -25,7 +25,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._diff import _dual
 from ._kernels import _ptr, _stream, _workspace
-from ._lib import FX_MAX_COLUMNS, FX_MAX_RADIUS, FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE, check, lib
+from ._lib import FX_MAX_BIAS_HEADS, FX_MAX_COLUMNS, FX_MAX_POSITIONS, FX_MAX_RADIUS, FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE, check, lib
 
 _TYPES = {torch.float32: _lib.FX_F32, torch.bfloat16: _lib.FX_BF16, torch.float16: _lib.FX_F16}
 _BIAS_TYPES = {**_TYPES, torch.float64: _lib.FX_F64}
@@ -180,7 +180,7 @@ def relative_bias(table, buckets, q_pos, k_pos):
 
         out[..., h, i, j] = table[bucket(k_pos[..., j] - q_pos[..., i]), h]
 
-    table (num_buckets, H) float32, float64, bfloat16 or float16, num_buckets <= 256; buckets from
+    table (num_buckets, H) float32, float64, bfloat16 or float16, num_buckets <= 256, H <= 4096; buckets from
     ``distance_buckets`` (entries past the table count as its last); q_pos (..., Q) and k_pos
     (..., K) int32 (or int64 values of its range), leading dimensions broadcast. As a pairing
     function of the electrons' distance the result goes straight into ``slogpf``. Differentiable in
@@ -190,6 +190,10 @@ def relative_bias(table, buckets, q_pos, k_pos):
     q, k = (_tensor(x, n, table, _INT) for x, n in ((q_pos, "q_pos"), (k_pos, "k_pos")))
     if not q.dim() or not k.dim():
         raise ValueError("q_pos and k_pos: expected (..., Q) and (..., K)")
+    if not 1 <= table.shape[1] <= FX_MAX_BIAS_HEADS:
+        raise ValueError(f"table: expected 1 to {FX_MAX_BIAS_HEADS} heads, got {table.shape[1]}")
+    if max(q.shape[-1], k.shape[-1]) > FX_MAX_POSITIONS:
+        raise ValueError(f"q_pos and k_pos: expected up to {FX_MAX_POSITIONS} positions, got {q.shape[-1]} and {k.shape[-1]}")
     _refuse_forward_mode(table)
     _on_device(table)
     lead = q.shape[:-1]

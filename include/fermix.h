@@ -473,12 +473,15 @@ int fx_det_parts_c128(const double* a, int64_t batch, int32_t n, double* sign, d
  *   out[b][h][i][j] = table[bucket(k_pos[b][j] - q_pos[b][i])][h],
  *   bucket(d) = min(map[clamp(d, -radius, radius) + radius], buckets - 1),
  * table (buckets, heads), out (batch, heads, nq, nk), both of dtype (any of the four),
- * contiguous; map 2 radius + 1 bytes, 0 <= radius <= FX_MAX_RADIUS; 1 <= buckets <= 256;
+ * contiguous; map 2 radius + 1 bytes, 0 <= radius <= FX_MAX_RADIUS; 1 <= buckets <= 256; heads up to
+ * FX_MAX_BIAS_HEADS, nq and nk up to FX_MAX_POSITIONS;
  * q_pos (batch, nq) and k_pos (batch, nk) any int32 (the distance saturates). Pointers are
  * aligned to their element. fx_relative_bias_grad: grad_table (buckets, heads) of dtype, the
  * sum of grad_out over the pairs of each bucket, in float32 (float64 for float64), in an
  * order that depends on the sizes alone. */
 #define FX_MAX_RADIUS 2048
+#define FX_MAX_BIAS_HEADS 4096
+#define FX_MAX_POSITIONS (1 << 30)
 int fx_relative_bias(const void* table, const uint8_t* map, int32_t radius, int32_t buckets, const int32_t* q_pos,
                      const int32_t* k_pos, int64_t batch, int32_t heads, int32_t nq, int32_t nk, int32_t dtype,
                      void* out, fx_stream_t stream);

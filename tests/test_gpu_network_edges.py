@@ -250,3 +250,26 @@ def test_norm_gate_shared_by_samples(dev, dtype, gc):
     network._call("fx_residual_norm_grad", y, ctypes.byref(s), ws.data_ptr(), size)
     near_sums(dg[:n].reshape(want["gate"].shape), want["gate"], want["size_gate"], dtype, dtype)
     assert (dg[n:] == 7.0).all()
+
+
+# ------------------------------------------------------------------ many heads
+
+
+@pytest.mark.parametrize("dtype", TYPES + [torch.float64], ids=ids)
+@pytest.mark.parametrize("nb,H,Q,K", [(256, 65, 9, 24), (256, 300, 5, 7), (32, 4096, 3, 4)])
+def test_relative_bias_many_heads(dev, dtype, nb, H, Q, K):
+    """Tables that no workgroup holds as a whole."""
+    gen = torch.Generator().manual_seed(H)
+    table, m = rand(gen, nb, H, dtype=dtype), fx.distance_buckets(nb, 200, device="cpu")
+    q, k = (torch.randint(-150, 150, (2, n), generator=gen).to(torch.int32) for n in (Q, K))
+    t = table.to(dev).requires_grad_(True)
+    out = fx.relative_bias(t, m.to(dev), q.to(dev), k.to(dev))
+    assert torch.equal(out.detach().double().cpu(), ref.relative_bias(table, m, q, k))
+    g = rand(gen, *out.shape, dtype=dtype)
+    (dt,) = torch.autograd.grad(out, t, g.to(dev))
+    bucket = ref.bucket_of(m, nb, q, k)
+    want, size = ref.bucket_sums(g.double(), bucket, nb), ref.bucket_sums(g.double().abs(), bucket, nb)
+    if dtype == torch.float64:
+        assert ((dt.cpu() - want).abs() <= 16 * U[dtype] * size).all()
+    else:
+        near_sums(dt, want, size, torch.float32, dtype)

@@ -45,3 +45,18 @@ def test_norm_gate_of_the_rows_alone():
     assert L.fx_residual_norm_grad(ctypes.byref(a), None, 0, None) == WORKSPACE
     a.gs, a.samples = 0, 1
     assert L.fx_residual_norm_grad(ctypes.byref(a), None, 0, None) == WORKSPACE
+
+
+def test_bias_limits():
+    """What the library cannot take is refused by name in Python, and by the C entry points."""
+    L = _lib.lib()
+    m, p = fx.distance_buckets(device="cpu"), torch.zeros(4, dtype=torch.int32)
+    for heads in (0, 4097):
+        with pytest.raises(ValueError, match="heads"):
+            fx.relative_bias(torch.zeros(32, heads), m, p, p)
+    with pytest.raises(fx.FermixDeviceError):
+        fx.relative_bias(torch.zeros(256, 4096), m, p, p)
+    with pytest.raises(ValueError, match="positions"):
+        fx.relative_bias(torch.zeros(32, 1), m, torch.zeros(1, dtype=torch.int32).expand(2**30 + 1), p)
+    for heads, nq, nk, want in ((4097, 0, 1, INVALID), (4096, 0, 1, OK), (1, 0, 2**30, OK), (1, 0, 2**30 + 1, INVALID), (1, 2**30 + 1, 0, INVALID)):
+        assert L.fx_relative_bias(None, None, 8, 4, None, None, 1, heads, nq, nk, _lib.FX_F32, None, None) == want
