@@ -122,6 +122,7 @@ FX_F32, FX_F64, FX_BF16, FX_F16 = 0, 1, 2, 3
 FX_MAX_RADIUS = 2048
 FX_MAX_BIAS_HEADS = 4096
 FX_MAX_POSITIONS = 1 << 30
+FX_MAX_STEP_TOKENS = 0x7FFFFF00
 FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE = 1, 2, 4
 FX_MAX_COLUMNS = 8192
 

@@ -681,7 +681,7 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
   const int group = p->heads / p->kv_heads, per = step_heads(*p);
   const int64_t rows = p->kv_heads * cdiv(group, per);
   const bool alone = p->batch * rows >= STEP_ALONE;
-  if (rows > 65535 || (int64_t)p->max_pages * p->page_size > 0x7fffff00 ||
+  if (rows > 65535 || (int64_t)p->max_pages * p->page_size > FX_MAX_STEP_TOKENS ||
       (int64_t)p->kv_heads * p->dim * p->page_size > 0xffffffffll)
     return FX_ERR_UNSUPPORTED;
 

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * W) void bias_grad_kernel(const BiasArgs a) {
 template <class T, class A>
 __global__ __launch_bounds__(BIAS_NT) void bucket_join_kernel(const A* part, int64_t n, int buckets, int heads,
                                                               T* out) {
-  const int t = blockIdx.x, h = blockIdx.y;
+  const int t = blockIdx.y, h = blockIdx.x;
   __shared__ double s[BIAS_NT];
   double x = 0.0;
   for (int64_t i = threadIdx.x; i < n; i += BIAS_NT) x += (double)part[((int64_t)h * n + i) * buckets + t];
@@ -209,7 +209,7 @@ bool bias_sizes_ok(int32_t radius, int32_t buckets, int64_t batch, int32_t heads
 }  // namespace
 
 int launch_bucket_join(const float* part, int64_t n, int buckets, int heads, float* out, hipStream_t s) {
-  hipLaunchKernelGGL((bucket_join_kernel<float, float>), dim3(buckets, heads), dim3(BIAS_NT), 0, s, part, n, buckets,
+  hipLaunchKernelGGL((bucket_join_kernel<float, float>), dim3(heads, buckets), dim3(BIAS_NT), 0, s, part, n, buckets,
                      heads, out);
   return launched();
 }
@@ -307,7 +307,7 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
       const int st = launched();
       if (st != FX_OK) return st;
     }
-    hipLaunchKernelGGL((bucket_join_kernel<T, A>), dim3(buckets, heads), dim3(BIAS_NT), 0, s,
+    hipLaunchKernelGGL((bucket_join_kernel<T, A>), dim3(heads, buckets), dim3(BIAS_NT), 0, s,
                        static_cast<const A*>(workspace), groups, buckets, heads, static_cast<T*>(grad_table));
     return launched();
   });

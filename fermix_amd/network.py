@@ -25,7 +25,10 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._diff import _dual
 from ._kernels import _ptr, _stream, _workspace
-from ._lib import FX_MAX_BIAS_HEADS, FX_MAX_COLUMNS, FX_MAX_POSITIONS, FX_MAX_RADIUS, FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE, check, lib
+from ._lib import (
+    FX_MAX_BIAS_HEADS, FX_MAX_COLUMNS, FX_MAX_POSITIONS, FX_MAX_RADIUS, FX_MAX_STEP_TOKENS, FX_NORM_LAYER, FX_NORM_POST,
+    FX_NORM_PRE, check, lib,
+)
 
 _TYPES = {torch.float32: _lib.FX_F32, torch.bfloat16: _lib.FX_BF16, torch.float16: _lib.FX_F16}
 _BIAS_TYPES = {**_TYPES, torch.float64: _lib.FX_F64}
@@ -317,6 +320,8 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     K = k.shape[1]
     if k.shape[0] != B:
         raise ValueError(f"q has {B} samples, k and v {k.shape[0]}")
+    if N > FX_MAX_POSITIONS or K > FX_MAX_POSITIONS:
+        raise ValueError(f"expected up to {FX_MAX_POSITIONS} queries and keys, got {N} and {K}")
     table, buckets = _check_bias(table, buckets, H, q)
     if (q_pos is None) != (k_pos is None):
         raise ValueError("q_pos and k_pos come together")
@@ -377,6 +382,8 @@ def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table
     _tensor(lengths, "lengths", q, _INT, 1)
     if pages.shape[0] != B or lengths.shape[0] != B:
         raise ValueError(f"pages {tuple(pages.shape)} and lengths {tuple(lengths.shape)} do not fit {B} samples")
+    if pages.shape[1] * page > FX_MAX_STEP_TOKENS or page * Hkv * D >= 2**32:
+        raise ValueError(f"expected pages of up to {FX_MAX_STEP_TOKENS} tokens for a sample, of less than 2^32 elements each")
     table, buckets = _check_bias(table, buckets, H, q)
     scale = _check_scale(scale, D)
     _refuse_forward_mode(q, k_cache, v_cache, k, v, table)

@@ -497,7 +497,7 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  *   left,  out = P v;  a query that no key is left for gets 0.
  * q, out: (batch, nq, heads, dim), k, v: (batch, nk, kv_heads, dim), heads a multiple of kv_heads
  * (head h reads kv head h / (heads / kv_heads)), 1 <= dim <= 128, dtype FX_F32, FX_BF16 or
- * FX_F16; own strides in elements for batch, token and head, dim contiguous. Scores, softmax
+ * FX_F16, nq and nk up to FX_MAX_POSITIONS; own strides in elements for batch, token and head, dim contiguous. Scores, softmax
  * and sums are float32; for the 16-bit types P (and dS) are rounded to dtype for the products (float16: brought up by
  * powers of two before, so that small weights and cotangents keep their digits).
  * Keys: index j < lengths[b] (NULL: nk), mask[b][j] != 0 (NULL: all; mask (batch, nk) bytes) and,
@@ -539,7 +539,8 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
 
 /* One token of each sample over a paged cache. The cache holds pages of page_size tokens, k_cache
  * and v_cache (pages, page_size, kv_heads, dim) packed; token t of sample b is in page
- * page_table[b][t / page_size] at t % page_size (page_table (batch, max_pages)). With k and v
+ * page_table[b][t / page_size] at t % page_size (page_table (batch, max_pages); max_pages page_size up to
+ * FX_MAX_STEP_TOKENS, the elements of a page below 2^32). With k and v
  * (batch, kv_heads, dim): they are stored as token lengths[b], and the query, at that position,
  * attends to tokens 0 .. lengths[b]; lengths[b] < 0 leaves a sample out. Without them the query
  * is at lengths[b] - 1 and attends to tokens 0 .. lengths[b] - 1. A sample with no token gets 0;
@@ -547,6 +548,7 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
  * stores nothing there. q, out (batch, heads, dim) packed. Types, heads, table, map as for
  * fx_attention. With several parts of the tokens at work (splits > 1 of the plan) the parts' sums
  * go through the workspace. Two samples must not name the same page for the token that they store. */
+#define FX_MAX_STEP_TOKENS 0x7fffff00
 typedef struct fx_attention_step {
   int64_t batch;
   int32_t heads, kv_heads, dim, dtype;

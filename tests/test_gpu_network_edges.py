@@ -273,3 +273,11 @@ def test_relative_bias_many_heads(dev, dtype, nb, H, Q, K):
         assert ((dt.cpu() - want).abs() <= 16 * U[dtype] * size).all()
     else:
         near_sums(dt, want, size, torch.float32, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_attention_many_heads(dev, dtype):
+    """More heads than a grid's second dimension holds."""
+    gen = torch.Generator().manual_seed(70000)
+    c = attention_case(gen, dtype, 1, 3, 4, 70000, 35000, 2, 4, 3)
+    check_attention(c, dev, dtype, gen)

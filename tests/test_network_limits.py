@@ -60,3 +60,25 @@ def test_bias_limits():
         fx.relative_bias(torch.zeros(32, 1), m, torch.zeros(1, dtype=torch.int32).expand(2**30 + 1), p)
     for heads, nq, nk, want in ((4097, 0, 1, INVALID), (4096, 0, 1, OK), (1, 0, 2**30, OK), (1, 0, 2**30 + 1, INVALID), (1, 2**30 + 1, 0, INVALID)):
         assert L.fx_relative_bias(None, None, 8, 4, None, None, 1, heads, nq, nk, _lib.FX_F32, None, None) == want
+
+
+def test_attention_lengths():
+    L = _lib.lib()
+    assert L.fx_attention_forward(attention(nq=2**30, nk=2**30, batch=0), None) == OK
+    for bad in (dict(nq=2**30 + 1), dict(nk=2**30 + 1)):
+        assert L.fx_attention_forward(attention(batch=0, **bad), None) == INVALID
+    x = torch.zeros(1, 1, 1, 8)
+    with pytest.raises(ValueError):
+        fx.attention(x, x.expand(1, 2**32 + 5, 1, 8), x.expand(1, 2**32 + 5, 1, 8))
+
+
+def test_step_pages():
+    """A table of more tokens than int32 counts, and a page of 2^32 elements: refused by name."""
+    q, n = torch.zeros(1, 1, 8), torch.zeros(1, dtype=torch.int32)
+    cache = torch.zeros(1, 1, 1, 8)
+    many = torch.zeros(1, 1, dtype=torch.int32).expand(1, 2**32 + 3)
+    with pytest.raises(ValueError, match="pages"):
+        fx.attention_step(q, cache, cache, many, n)
+    meta = torch.empty(1, 2**29, 1, 8, device="meta")
+    with pytest.raises(ValueError, match="pages"):
+        fx.attention_step(q.to("meta"), meta, meta, many[:, :1].to("meta"), n.to("meta"))
