@@ -123,6 +123,7 @@ FX_MAX_RADIUS = 2048
 FX_MAX_BIAS_HEADS = 4096
 FX_MAX_POSITIONS = 1 << 30
 FX_MAX_STEP_TOKENS = 0x7FFFFF00
+FX_MIN_SCALE, FX_MAX_SCALE = 1e-30, 1e30
 FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE = 1, 2, 4
 FX_MAX_COLUMNS = 8192
 

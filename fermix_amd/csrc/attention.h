@@ -100,6 +100,9 @@ __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float F32_MAX = 3.402823466e38f;
 
+// Scales whose reciprocal and product with log2 e are far from float32's ends (at which a bias of 0 would become NaN).
+inline bool scale_ok(float scale) { return scale >= FX_MIN_SCALE && scale <= FX_MAX_SCALE; }
+
 // A bias in the unit of the raw product q k (scores are c acc, c = scale log2 e): finite entries stay
 // finite, so that the type's lowest value weighs like any other and only -inf forbids.
 __device__ __forceinline__ float scaled_bias(float b, float inv_scale) {

@@ -148,7 +148,7 @@ bool attention_sizes_ok(const fx_attention* p) {
       p->dim < 1 || p->dim > 128)
     return false;
   if (p->dtype != FX_F32 && p->dtype != FX_BF16 && p->dtype != FX_F16) return false;
-  if (!(p->scale > 0.0f) || !(p->scale <= F32_MAX)) return false;
+  if (!scale_ok(p->scale)) return false;
   if (p->offset < 0 || p->offset > 0x7fffffff - (p->nq > p->nk ? p->nq : p->nk)) return false;
   if (p->table ? p->buckets < 1 || p->buckets > FX_MAX_ATTENTION_BUCKETS || p->radius < 0 || p->radius > FX_MAX_RADIUS
                : p->buckets != 0 || p->radius != 0)

@@ -616,7 +616,7 @@ bool step_sizes_ok(const fx_attention_step* p) {
       p->pages < 0 || p->page_size < 1 || p->max_pages < 0)
     return false;
   if (p->dtype != FX_F32 && p->dtype != FX_BF16 && p->dtype != FX_F16) return false;
-  if (!(p->scale > 0.0f) || !(p->scale <= F32_MAX)) return false;
+  if (!scale_ok(p->scale)) return false;
   return p->table ? p->buckets >= 1 && p->buckets <= FX_MAX_ATTENTION_BUCKETS && p->radius >= 0 && p->radius <= FX_MAX_RADIUS
                   : p->buckets == 0 && p->radius == 0;
 }

@@ -26,8 +26,8 @@ from . import _lib
 from ._diff import _dual
 from ._kernels import _ptr, _stream, _workspace
 from ._lib import (
-    FX_MAX_BIAS_HEADS, FX_MAX_COLUMNS, FX_MAX_POSITIONS, FX_MAX_RADIUS, FX_MAX_STEP_TOKENS, FX_NORM_LAYER, FX_NORM_POST,
-    FX_NORM_PRE, check, lib,
+    FX_MAX_BIAS_HEADS, FX_MAX_COLUMNS, FX_MAX_POSITIONS, FX_MAX_RADIUS, FX_MAX_SCALE, FX_MAX_STEP_TOKENS, FX_MIN_SCALE,
+    FX_NORM_LAYER, FX_NORM_POST, FX_NORM_PRE, check, lib,
 )
 
 _TYPES = {torch.float32: _lib.FX_F32, torch.bfloat16: _lib.FX_BF16, torch.float16: _lib.FX_F16}
@@ -288,8 +288,8 @@ def _check_bias(table, buckets, heads, like):
 
 def _check_scale(scale, dim):
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not (0.0 < scale < 3e38):
-        raise ValueError(f"scale: expected a positive finite number, got {scale}")
+    if not FX_MIN_SCALE <= scale <= FX_MAX_SCALE:
+        raise ValueError(f"scale: expected {FX_MIN_SCALE} to {FX_MAX_SCALE}, got {scale}")
     return scale
 
 
@@ -307,7 +307,7 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     lengths (B,): keys at or past it are left out; mask (B, K) bool: keys that are False are; both may
     hide anything, NaN and infinities included. causal: query i sees keys j <= offset + i (what is
     hidden by it alone has to be finite). q_lengths (B,): queries at or past it give 0. A query with no key
-    gives 0 and no gradient. An entry -inf of table forbids its bucket. scale defaults to
+    gives 0 and no gradient. An entry -inf of table forbids its bucket. scale, 1e-30 to 1e30, defaults to
     1 / sqrt(D).
 
     Differentiable in q, k, v and table. The gradient keeps q, k, v, out and two float32 a query and

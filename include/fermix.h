@@ -505,7 +505,8 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * value that causal alone masks has to be finite. Queries i >= q_lengths[b] (NULL: nq) get 0
  * and no gradient. Positions: q_pos (batch, nq), k_pos (batch, nk) together, or NULL: offset + i
  * and j; 0 <= offset <= 2^31 - 1 - max(nq, nk). table (buckets, heads) float32 or NULL (no bias), map and radius as above, buckets <= FX_MAX_ATTENTION_BUCKETS;
- * its entries may be -inf, and entries of float32's lowest value weigh like any other.
+ * its entries may be -inf; finite ones past scale x float32's largest value count as that, so that entries of
+ * float32's lowest value weigh like any other.
  *
  * fx_attention_forward: out and, if given, stats (batch, heads, nq, 2): the largest S / scale and log2
  * of the sum of exp(S - its maximum); 0 and +inf where there is no key. With fx_attention_keeps_low(p) != 0 a
@@ -515,11 +516,13 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * tensors) and grad_table (buckets, heads) float32 (NULL to skip) from grad_out (packed), out
  * (packed), stats and out_low. Deterministic: sums are in an order that depends on sizes alone. */
 #define FX_MAX_ATTENTION_BUCKETS 64
+#define FX_MIN_SCALE 1e-30f
+#define FX_MAX_SCALE 1e30f
 typedef struct fx_attention {
   int64_t batch;
   int32_t nq, nk, heads, kv_heads, dim, dtype;
   int32_t causal, offset, radius, buckets;
-  float scale; /* finite, > 0 */
+  float scale; /* FX_MIN_SCALE .. FX_MAX_SCALE */
   const void *q, *k, *v;
   int64_t qb, qn, qh, kb, kn, kh, vb, vn, vh;
   const float* table;

@@ -281,3 +281,24 @@ def test_attention_many_heads(dev, dtype):
     gen = torch.Generator().manual_seed(70000)
     c = attention_case(gen, dtype, 1, 3, 4, 70000, 35000, 2, 4, 3)
     check_attention(c, dev, dtype, gen)
+
+
+# ------------------------------------------------------------------ the smallest and the largest scale
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e12, 1e30])
+def test_attention_scales(dev, dtype, scale):
+    """A scale at which the table alone decides (its entries of 0 among them), or the largest product does."""
+    gen = torch.Generator().manual_seed(5)
+    for mode in ("", "p"):
+        c = attention_case(gen, dtype, 1, 70, 90, 2, 1, 32, mode=mode)
+        c["table"][::3] = 0.0
+        c["scale"] = scale
+        near(run_attention(c, dev), ref.attention(**c), dtype, 2, (scale, mode))
+    q, k, v = (c[n].to(dev) for n in "qkv")
+    pages = torch.arange(9, dtype=torch.int32, device=dev)[None]
+    out = fx.attention_step(q[:, 0], k.reshape(9, 10, 1, 32), v.reshape(9, 10, 1, 32), pages, torch.tensor([90], dtype=torch.int32, device=dev),
+                            table=c["table"].to(dev), buckets=c["buckets"].to(dev), scale=scale)
+    want = ref.attention(c["q"][:, :1], c["k"], c["v"], c["table"], c["buckets"], offset=89, scale=scale)
+    near(out, want[:, 0], dtype, 2, (scale, "step"))

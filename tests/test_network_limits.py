@@ -82,3 +82,23 @@ def test_step_pages():
     meta = torch.empty(1, 2**29, 1, 8, device="meta")
     with pytest.raises(ValueError, match="pages"):
         fx.attention_step(q.to("meta"), meta, meta, many[:, :1].to("meta"), n.to("meta"))
+
+
+def test_scales():
+    L = _lib.lib()
+    x, k = torch.zeros(1, 2, 1, 8), torch.zeros(1, 1, 1, 8)
+    p, n = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+    def step(scale):
+        return L.fx_attention_step_run(ctypes.byref(_lib.FxAttentionStep(batch=0, heads=1, kv_heads=1, dim=8, page_size=1, scale=scale)), None, 0, None)
+
+    for scale in (1e-30, 1e30):
+        assert L.fx_attention_forward(attention(scale=scale, batch=0), None) == OK and step(scale) == OK
+        with pytest.raises(fx.FermixDeviceError):
+            fx.attention(x, x, x, scale=scale)
+    for bad in (0.0, -1.0, 1e-45, 9e-31, 1.1e30, 3e38, float("inf"), float("nan")):
+        assert L.fx_attention_forward(attention(scale=bad, batch=0), None) == INVALID and step(bad) == INVALID
+        with pytest.raises(ValueError, match="scale"):
+            fx.attention(x, x, x, scale=bad)
+        with pytest.raises(ValueError, match="scale"):
+            fx.attention_step(x[0], k, k, p, n, scale=bad)
