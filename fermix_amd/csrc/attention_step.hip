@@ -727,12 +727,16 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
                              dim3(STEP_NT), STEP_WAVES * G * (4 * DP + 8) + tab + map, s, c);
       };
       auto by_heads = [&](auto dp) {
-        if (per == 1)
+        if constexpr (sizeof(T) == 2) {  // heads that share K and V are above
           go(dp, ic<1>{});
-        else if (per == 2)
-          go(dp, ic<2>{});
-        else
-          go(dp, ic<4>{});
+        } else {
+          if (per == 1)
+            go(dp, ic<1>{});
+          else if (per == 2)
+            go(dp, ic<2>{});
+          else
+            go(dp, ic<4>{});
+        }
       };
       if constexpr (sizeof(T) == 2) {
         if (step_mma(*p)) {
