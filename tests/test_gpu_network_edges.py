@@ -222,6 +222,31 @@ def test_traces_replay_on_other_inputs(dev):
         torch.jit.trace(lambda q: fx.attention_step(q, cache, cache.clone(), z, z[:, 0]), (torch.randn(2, 4, 16, device=dev),))
 
 
+@pytest.mark.parametrize("transform", ["jvp", "vmap", "grad", "jacrev", "vmap of grad"])
+@pytest.mark.parametrize("name", ["relative_bias", "attention", "residual_norm", "attention_step"])
+def test_function_transforms_raise(dev, name, transform):
+    """torch.func sees tensors that are not the caller's: every operator raises under each of them."""
+    m, p = fx.distance_buckets(device=dev), torch.arange(4, dtype=torch.int32, device=dev)
+    q, z = torch.randn(2, 4, 2, 8, device=dev), torch.zeros(2, 1, dtype=torch.int32, device=dev)
+    cache = torch.zeros(2, 4, 2, 8, device=dev)
+    f, x = {
+        "relative_bias": (lambda t: fx.relative_bias(t, m, p, p), torch.randn(32, 2, device=dev)),
+        "attention": (lambda t: fx.attention(t, q, q), q.clone()),
+        "residual_norm": (lambda t: fx.residual_norm(t, 2 * q)[0], q.clone()),
+        "attention_step": (lambda t: fx.attention_step(t, cache, cache, z, z[:, 0]), torch.randn(2, 2, 8, device=dev)),
+    }[name]
+    run = {
+        "jvp": lambda: torch.func.jvp(f, (x,), (torch.ones_like(x),)),
+        "vmap": lambda: torch.func.vmap(f)(torch.stack([x, x])),
+        "grad": lambda: torch.func.grad(lambda t: f(t).sum())(x),
+        "jacrev": lambda: torch.func.jacrev(f)(x),
+        "vmap of grad": lambda: torch.func.vmap(torch.func.grad(lambda t: f(t).sum()))(torch.stack([x, x])),
+    }[transform]
+    f(x)
+    with pytest.raises(RuntimeError):
+        run()
+
+
 # ------------------------------------------------------------------ the C entry points' own layouts
 
 
