@@ -111,14 +111,19 @@ __device__ __forceinline__ float scaled_bias(float b, float inv_scale) {
 }
 
 // float16 loses digits below 2^-14 and has nothing below 2^-25, where weights of long rows lie (some 1 / keys, and beside
-// a dominant key far less) and dS of a small cotangent. Its weights are formed as 2^WEIGHT_SHIFT exp(..), at most
-// 2^15, which costs nothing in the exponent, and dS are brought up by a power of two (fit_scale).
+// a dominant key far less) and dS of a small cotangent. Its weights, at most 1, are rounded as 2^15 of them (in
+// units of WEIGHT_UNIT), and dS are brought up by a power of two (fit_scale). A product for each weight: 4 % of a long
+// forward (699 -> 726 us at 2 x 16 heads x 8192, head dimension 128). In the exponent the 15 would cost nothing, but
+// rounds it at 2^-20, which doubled the error of d table.
 template <class T>
 constexpr bool IS_F16 = __is_same(T, _Float16);
 template <class T>
-constexpr int WEIGHT_SHIFT = IS_F16<T> ? 15 : 0;
-template <class T>
 constexpr float WEIGHT_UNIT = IS_F16<T> ? 0x1p-15f : 1.0f;
+template <class T>
+__device__ __forceinline__ v16f in_units(const v16f& weights) {
+  if constexpr (IS_F16<T>) return weights * (1.0f / WEIGHT_UNIT<T>);
+  return weights;
+}
 
 // The power of two that brings top to [2^(to - 1), 2^to), at most 2^100; 2^to for 0 and what is not finite.
 __device__ __forceinline__ float power_to(float top, int to) {
@@ -127,8 +132,9 @@ __device__ __forceinline__ float power_to(float top, int to) {
 
 // Scale of a lane's column of dS for a float16 product: dS f is at most 2^15. Starts at SCALE_START and comes down where
 // a block's largest asks for it, and what has been summed with it: once for most rows, as it then leaves a factor of 2
-// to 4. What is below the largest by 2^-28 keeps its digits. Costs 7 % of a long gradient (3404 -> 3650 us at 2 x 16 heads x
-// 8192, head dimension 128; 1 % for short sequences), without it dk of cotangents of 1e-4 was 3 % off.
+// to 4. What is below the largest by 2^-28 keeps its digits. A call with gradients takes 8 % more (3390 -> 3660 us at 2 x 16
+// heads x 8192, head dimension 128; 2 % for short sequences), of which the weights' units are a tenth; without it dk of
+// cotangents of 1e-4 was 3 % off.
 constexpr float SCALE_START = 0x1p60f;
 template <int DB>
 __device__ __forceinline__ void fit_scale(float& f, const v16f& ds, v16f (&acc)[DB]) {
@@ -145,20 +151,14 @@ __device__ __forceinline__ void fit_scale(float& f, const v16f& ds, v16f (&acc)[
   }
 }
 
-// 2^WEIGHT_SHIFT exp2(c (s - m)) for a block of raw scores; base is c m - WEIGHT_SHIFT. One fma each while c m is small;
-// past BASE_MAX (entries of the table like the type's lowest value), where c m's own rounding would be a factor, and
-// always for float32, the difference is formed first.
+// exp2(c (s - m)) for a block of raw scores. One fma each while c m is small; past BASE_MAX (entries of the
+// table like the type's lowest value), where c m's own rounding would be a factor, and always for float32,
+// the difference is formed first.
 constexpr float BASE_MAX = 1024.0f;
-template <class T>
 __device__ __forceinline__ void exp_block(v16f& s, float c, float m, float base, bool exact) {
   if (exact) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (IS_F16<T>)
-        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i] - m, c, (float)WEIGHT_SHIFT<T>));
-      else
-        s[i] = __builtin_amdgcn_exp2f((s[i] - m) * c);
-    }
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f((s[i] - m) * c);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -base));

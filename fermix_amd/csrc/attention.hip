@@ -105,7 +105,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
     }
     const float next = fmaxf(m, half_max(top));
-    const float ref = next == -INFINITY ? 0.0f : next, base = ref * a.c - WEIGHT_SHIFT<T>;
+    const float ref = next == -INFINITY ? 0.0f : next, base = ref * a.c;
     const bool exact = sizeof(T) == 4 || __any(fabsf(base) > BASE_MAX);
     const float keep = __builtin_amdgcn_exp2f(exact ? (m - ref) * a.c : m_base - base);
     m = next;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
     float sum = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      exp_block<T>(s[kb], a.c, ref, base, exact);
+      exp_block(s[kb], a.c, ref, base, exact);
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum += s[kb][i];
     }
@@ -123,12 +123,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
       for (int d = 0; d < DB; ++d) o[d] *= keep;
     }
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) column_product<T, DP>(vt, 32 * kb, s[kb], o, lane, p.dim);
+    for (int kb = 0; kb < 2; ++kb) column_product<T, DP>(vt, 32 * kb, in_units<T>(s[kb]), o, lane, p.dim);
   }
 
   const bool out_in = qi < p.nq;
   l = half_sum(l);
-  const float inv = l > 0.0f ? 1.0f / l : (l != l ? l : 0.0f);
+  const float inv = l > 0.0f ? WEIGHT_UNIT<T> / l : (l != l ? l : 0.0f);
   const int64_t row = (at.b * p.nq + qi) * p.heads + at.h;
   store_rows<T, DP>(static_cast<T*>(p.out) + row * p.dim, out_in, o, inv, p.dim, a.whole, half);
   if constexpr (sizeof(T) == 2)
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * (int)sizeof(T) <= 256 ? 2 : 1) voi
       store_low<T, DP>(static_cast<_Float16*>(p.out_low) + row * p.dim, out_in, o, inv, p.dim, a.whole, half);
   if (p.stats && out_in && half == 0)
     reinterpret_cast<float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi] =
-        l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l * WEIGHT_UNIT<T>));
+        l == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(l));
 }
 
 int forward_waves(const fx_attention& p) { return p.dim > 64 && p.dtype != FX_F32 && p.nq > 128 ? 8 : 4; }

@@ -262,7 +262,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
     sum[0][d] = v16f{};
     if (!SPLIT) sum[SPLIT ? 0 : 1][d] = v16f{};
   }
-  float fit = IS_F16<T> ? SCALE_START : 1.0f;  // of 2^WEIGHT_SHIFT dS
+  float fit = IS_F16<T> ? SCALE_START : 1.0f;
   // queries that some key of the workgroup is seen by
   const int first = p.causal ? max(0, k0 - p.offset) / ATT_TILE * ATT_TILE : 0;
   const int queries = k0 < klen ? qlen : 0;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
       if (threadIdx.x < ATT_TILE) {
         const bool exact = sizeof(T) == 4 || __any(fabsf(ml.x * a.c) > BASE_MAX);
         qv.max[threadIdx.x] = ml.x;
-        qv.log[threadIdx.x] = (exact ? ml.y : ml.x * a.c + ml.y) - WEIGHT_SHIFT<T>;
+        qv.log[threadIdx.x] = exact ? ml.y : ml.x * a.c + ml.y;
         if (threadIdx.x == 0) *qv.exact = exact;
         qv.delta[threadIdx.x] = de;
         if (GEN) qv.pos[threadIdx.x] = qp;
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = in ? s[i] : 0.0f;
         }
-        if (do_v) column_product<T, DP>(gt, 32 * qb, s, sum[SPLIT ? 0 : 1], lane, p.dim);
+        if (do_v) column_product<T, DP>(gt, 32 * qb, in_units<T>(s), sum[SPLIT ? 0 : 1], lane, p.dim);
         if (!do_k) continue;
         const v16f dp = row_product<T, DP>(gt, 32 * qb, v, v16f{}, lane, p.dim);
 #pragma unroll
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, sizeof(T) == 2 || DP == 32 ? 2 :
   }
   const int64_t row = ((at.b * p.nk + ki) * p.kv_heads + at.h) * p.dim;
   if (do_k)
-    store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, sum[0], p.scale * WEIGHT_UNIT<T> / fit, p.dim, a.whole, half);
+    store_rows<T, DP>(static_cast<T*>(p.grad_k) + row, ki < p.nk, sum[0], p.scale / fit, p.dim, a.whole, half);
   if (do_v)
     store_rows<T, DP>(static_cast<T*>(p.grad_v) + row, ki < p.nk, sum[SPLIT ? 0 : 1], WEIGHT_UNIT<T>, p.dim, a.whole, half);
 }

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
     for (int t = 0; t < p.buckets; ++t) sums.ds[64 * t] = 0.0f;
   const float2 ml = in ? reinterpret_cast<const float2*>(p.stats)[(at.b * p.heads + at.h) * p.nq + qi]
                        : make_float2(0.0f, INFINITY);
-  const float log = ml.y - WEIGHT_SHIFT<T>, base = ml.x * a.c + log;
+  const float base = ml.x * a.c + ml.y;
   const bool exact = __any(fabsf(ml.x * a.c) > BASE_MAX);
   __syncthreads();
   if (!GEN) {
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
     __syncthreads();
   }
 
-  // P (float16: times 2^WEIGHT_SHIFT, also in dS) and dP of all keys, delta
+  // P and dP of all keys, delta
   const int64_t last = !in ? 0 : p.causal ? min((int64_t)klen, (int64_t)p.offset + qi + 1) : (int64_t)klen;
   v16f s[4], dp[4];
   float delta = 0.0f;
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
     dp[kb] = row_product<T, DP>(t1, 32 * kb, g, dp[kb], lane, p.dim);
     if (exact) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i] - ml.x, a.c, -log));
+      for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i] - ml.x, a.c, -ml.y));
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.c, -base));
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
 #pragma unroll
     for (int i = 0; i < 16; ++i) delta += s[kb][i] * dp[kb][i];
   }
-  delta = half_sum(delta) * WEIGHT_UNIT<T>;
+  delta = half_sum(delta);
 
   // float16: dS scaled so that the head's largest is just below 2^15. (A scale for each query would serve dq alone: dk's
   // products are over the queries.)
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
 #pragma unroll
   for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) pr[kb][i] = M::from_acc(s[kb], i);
+    for (int i = 0; i < 2; ++i) pr[kb][i] = M::from_acc(in_units<T>(s[kb]), i);
 #pragma unroll
     for (int i = 0; i < 16; ++i) dp[kb][i] = s[kb][i] * (dp[kb][i] - delta);
     const v16f ds = IS_F16<T> ? dp[kb] * fit : dp[kb];
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
       bucket_add<GEN>(bv, KeyView{kpos + k0, nullptr}, sums, dp[kb], s[kb], kb & 1, k0, qpos, half, far[kb / 2], false);
     column_product<T, DP>(t0, 32 * kb, ds, dq, lane, p.dim);
   }
-  const float unit = p.scale * WEIGHT_UNIT<T> / fit;  // of dq and dk
+  const float unit = p.scale / fit;  // of dq and dk
   store_rows<T, DP>(static_cast<T*>(p.grad_q) + row * p.dim, qi < p.nq, dq, unit, p.dim, a.whole, half);
   if (!GEN && p.grad_table) add_pair(sums.ds, bv.map[0], sums.far_ds[0], bv.map[2 * p.radius + 128], sums.far_ds[1]);
   __syncthreads();
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(SHORT_NT, DP <= 64 ? 2 : 1) void attention_short_gr
 #pragma unroll 8
       for (int l = 0; l < 64; ++l) x += w[(l + threadIdx.x) & 63];  // rotated: no shared bank
       x = group_sum<SHORT_WAVES>(x);
-      if (threadIdx.x % SHORT_WAVES == 0) out[t] = x * WEIGHT_UNIT<T>;
+      if (threadIdx.x % SHORT_WAVES == 0) out[t] = x;
     }
   }
 

@@ -489,11 +489,9 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float d = s[t][r] - ref;
-        if constexpr (IS_F16<T>) d += WEIGHT_SHIFT<T>;  // leaves the result, and the sums it is joined with, by l
-        const float x = __builtin_amdgcn_exp2f(d);
+        const float x = __builtin_amdgcn_exp2f(s[t][r] - ref);
         sum += x;
-        w[4 * t + r] = (T)x;
+        w[4 * t + r] = (T)(x * (1.0f / WEIGHT_UNIT<T>));
       }
     l = l * keep + sum;
     if (__any(keep != 1.0f)) {
@@ -513,7 +511,7 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
   if constexpr (W == 1) {
     bad = __any(bad);
     if (spare || c >= heads) return;
-    const float inv = bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = bad ? NAN : l == 0.0f ? 0.0f : WEIGHT_UNIT<T> / l;
     T* const out = static_cast<T*>(p.out) + (b * p.heads + h0 + c) * p.dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
@@ -538,7 +536,7 @@ __global__ __launch_bounds__(STEP_NT, 2) void step_mma_kernel(const StepArgs a) 
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc_lds[(wave * heads + c) * R + 16 * d + 4 * g + r] = o[d][r];
+        for (int r = 0; r < 4; ++r) acc_lds[(wave * heads + c) * R + 16 * d + 4 * g + r] = o[d][r] * WEIGHT_UNIT<T>;
       if (g == 0) stat_lds[wave * heads + c] = make_float2(m, l);
     }
     __syncthreads();
