@@ -10,9 +10,12 @@ HIP kernels of ``libfermix_amd.so``; there is no CPU path.
   with their gradients.
 
 Element types are float32, bfloat16 and float16 (``relative_bias`` also float64); scores,
-statistics and sums are held in float32 and each result is rounded once. Every result is
-deterministic. Gradients are reverse mode, once (``torch.autograd``); forward mode and
-``torch.func`` transforms raise.
+statistics and sums are held in float32 and each result is rounded once. For the 16-bit types attention's
+weights (and what its gradient makes of them) are rounded to the type a first time, as an operand of
+the next product. Every result is deterministic: its sums are in an order that depends on sizes and
+lengths, for the bias' gradient and the float32 norms also on the tensors' alignment to 16 bytes.
+Gradients are reverse mode, once (``torch.autograd``); forward mode and ``torch.func`` transforms raise.
+``torch.jit.trace`` records calls, but for ``attention_step``.
 """
 
 import ctypes
@@ -307,8 +310,12 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     lengths (B,): keys at or past it are left out; mask (B, K) bool: keys that are False are; both may
     hide anything, NaN and infinities included. causal: query i sees keys j <= offset + i (what is
     hidden by it alone has to be finite). q_lengths (B,): queries at or past it give 0. A query with no key
-    gives 0 and no gradient. An entry -inf of table forbids its bucket. scale, 1e-30 to 1e30, defaults to
-    1 / sqrt(D).
+    gives 0 and no gradient (its cotangent has to be finite). An entry -inf of table forbids its bucket. scale,
+    1e-30 to 1e30, defaults to 1 / sqrt(D).
+
+    For bfloat16 and float16 the softmax' weights are rounded to the type for their product with v, and dS in the
+    gradient likewise: out, dq, dk and dv have up to 1.5 times the error of one rounding. (float16's are scaled by powers
+    of two before, so that small weights and cotangents keep their digits.)
 
     Differentiable in q, k, v and table. The gradient keeps q, k, v, out and two float32 a query and
     head; for 16-bit types past 128 queries or keys also what out lost to rounding, as float16."""
@@ -360,7 +367,8 @@ def attention_step(q, k_cache, v_cache, pages, lengths, *, k=None, v=None, table
     of the cache's last token. table, buckets and scale as for ``attention``; a key's distance
     is its token less the query's. Samples may share pages that they only read (walkers that branched).
     A sample with no token gives 0; one that its row of pages cannot hold, or that names a page outside
-    the cache, gives NaN. No gradient."""
+    the cache, gives NaN. For bfloat16 and float16 with shared key heads the weights are rounded to the type, as in
+    ``attention``. No gradient."""
     _tensor(q, "q", dtype=_TYPES, dim=3)
     for x, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _tensor(x, name, q, (q.dtype,), 4)

@@ -478,7 +478,7 @@ int fx_det_parts_c128(const double* a, int64_t batch, int32_t n, double* sign, d
  * q_pos (batch, nq) and k_pos (batch, nk) any int32 (the distance saturates). Pointers are
  * aligned to their element. fx_relative_bias_grad: grad_table (buckets, heads) of dtype, the
  * sum of grad_out over the pairs of each bucket, in float32 (float64 for float64), in an
- * order that depends on the sizes alone. */
+ * order that depends on the sizes and on grad_out's alignment to 16 bytes alone. */
 #define FX_MAX_RADIUS 2048
 #define FX_MAX_BIAS_HEADS 4096
 #define FX_MAX_POSITIONS (1 << 30)
@@ -504,8 +504,8 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * with causal, j <= offset + i. What is masked by lengths or mask may hold anything; a
  * value that causal alone masks has to be finite. Queries i >= q_lengths[b] (NULL: nq) get 0
  * and no gradient. Positions: q_pos (batch, nq), k_pos (batch, nk) together, or NULL: offset + i
- * and j; 0 <= offset <= 2^31 - 1 - max(nq, nk). table (buckets, heads) float32 or NULL (no bias), map and radius as above, buckets <= FX_MAX_ATTENTION_BUCKETS;
- * its entries may be -inf; finite ones past scale x float32's largest value count as that, so that entries of
+ * and j; 0 <= offset <= 2^31 - 1 - max(nq, nk). table (buckets, heads) float32 or NULL (no bias), map and radius as
+ * above, buckets <= FX_MAX_ATTENTION_BUCKETS; its entries may be -inf; finite ones past scale x float32's largest value count as that, so that entries of
  * float32's lowest value weigh like any other.
  *
  * fx_attention_forward: out and, if given, stats (batch, heads, nq, 2): the largest S / scale and log2
@@ -514,7 +514,7 @@ int fx_relative_bias_grad(const void* grad_out, const uint8_t* map, int32_t radi
  * or 2048 (float16), without which dq has up to 6 % more error (NULL: not written, not read).
  * fx_attention_grad: grad_q, grad_k, grad_v (strides of their own: those of q, k, v in packed
  * tensors) and grad_table (buckets, heads) float32 (NULL to skip) from grad_out (packed), out
- * (packed), stats and out_low. Deterministic: sums are in an order that depends on sizes alone. */
+ * (packed), stats and out_low. Deterministic: sums are in an order that depends on sizes and lengths alone. */
 #define FX_MAX_ATTENTION_BUCKETS 64
 #define FX_MIN_SCALE 1e-30f
 #define FX_MAX_SCALE 1e30f
@@ -548,9 +548,9 @@ int fx_attention_grad(const fx_attention* p, void* workspace, size_t workspace_b
  * attends to tokens 0 .. lengths[b]; lengths[b] < 0 leaves a sample out. Without them the query
  * is at lengths[b] - 1 and attends to tokens 0 .. lengths[b] - 1. A sample with no token gets 0;
  * one whose tokens pass its table, or whose table names a page outside the cache, gets NaN and
- * stores nothing there. q, out (batch, heads, dim) packed. Types, heads, table, map as for
- * fx_attention. With several parts of the tokens at work (splits > 1 of the plan) the parts' sums
- * go through the workspace. Two samples must not name the same page for the token that they store. */
+ * stores nothing there. q, out (batch, heads, dim) packed. Types, heads, table, map, scale as for
+ * fx_attention; the weights are rounded to a 16-bit dtype where heads share K and V. With several parts of the tokens
+ * at work (splits > 1 of the plan) the parts' sums go through the workspace. Two samples must not name the same page for the token that they store. */
 #define FX_MAX_STEP_TOKENS 0x7fffff00
 typedef struct fx_attention_step {
   int64_t batch;
@@ -582,7 +582,8 @@ int fx_attention_step_run(const fx_attention_step* p, void* workspace, size_t wo
  * broadcast). x, h, gate, y, z, cotangents and their gradients have dtype (FX_F32, FX_BF16,
  * FX_F16); weights, biases and scale (columns), each optional (NULL: 1 or 0), have wdtype,
  * which is dtype or FX_F32. stats: 4 floats a row (mean and reciprocal deviation of h, then of
- * y), written by the forward if given, read by the gradient. 1 <= columns <= FX_MAX_COLUMNS. */
+ * y), written by the forward if given, read by the gradient. 1 <= columns <= FX_MAX_COLUMNS. Sums are in an order that
+ * depends on the sizes and, for FX_F32, on the rows' alignment to 16 bytes alone. */
 #define FX_NORM_LAYER 1
 #define FX_NORM_POST 2
 #define FX_NORM_PRE 4
