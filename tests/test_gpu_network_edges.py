@@ -20,15 +20,16 @@ pytestmark = pytest.mark.gpu
 # ------------------------------------------------------------------ nothing to work on
 
 
+EMPTY = [(0, 5, 16), (5, 0, 16), (0, 1, 16), (0, 16), (3, 0, 2, 16), (0, 5, 300)]
+WITH_ELEMENTS = [(s, g) for s in EMPTY for g in GATES if GATES[g](s) is not None and math.prod(GATES[g](s))]
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
-@pytest.mark.parametrize("gate", GATES)
-@pytest.mark.parametrize("shape", [(0, 5, 16), (5, 0, 16), (0, 1, 16), (0, 16), (3, 0, 2, 16), (0, 5, 300)], ids=lambda s: "x".join(map(str, s)))
-def test_norm_gate_without_rows(dev, dtype, gate, shape):
+@pytest.mark.parametrize("shape,gate", WITH_ELEMENTS, ids=lambda s: s if isinstance(s, str) else "x".join(map(str, s)))
+def test_norm_gate_without_rows(dev, dtype, shape, gate):
     """Without rows every gradient is zero, a broadcast gate's too, which has elements all the same; the
     allocator's memory is filled with NaN beforehand, so that a result that nobody writes shows."""
     s = GATES[gate](shape)
-    if s is None or math.prod(torch.Size(s)) == 0:
-        pytest.skip("no gate, or one without elements")
     x, h = (torch.zeros(shape, dtype=dtype, device=dev, requires_grad=True) for _ in range(2))
     g = torch.ones(s, dtype=dtype, device=dev, requires_grad=True)
     w = torch.ones(shape[-1], device=dev, requires_grad=True)
