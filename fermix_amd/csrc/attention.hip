@@ -144,8 +144,8 @@ int forward_waves(const fx_attention& p) { return p.dim > 64 && p.dtype != FX_F3
 }  // namespace
 
 bool attention_sizes_ok(const fx_attention* p) {
-  if (!p || p->batch < 0 || p->nq < 0 || p->nq > FX_MAX_POSITIONS || p->nk < 0 || p->nk > FX_MAX_POSITIONS || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads ||
-      p->dim < 1 || p->dim > 128)
+  if (!p || p->batch < 0 || p->nq < 0 || p->nq > FX_MAX_POSITIONS || p->nk < 0 || p->nk > FX_MAX_POSITIONS ||
+      p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->dim < 1 || p->dim > 128)
     return false;
   if (p->dtype != FX_F32 && p->dtype != FX_BF16 && p->dtype != FX_F16) return false;
   if (!scale_ok(p->scale)) return false;

@@ -314,8 +314,8 @@ def attention(q, k, v, *, table=None, buckets=None, q_pos=None, k_pos=None, leng
     1e-30 to 1e30, defaults to 1 / sqrt(D).
 
     For bfloat16 and float16 the softmax' weights are rounded to the type for their product with v, and dS in the
-    gradient likewise: out, dq, dk and dv have up to 1.5 times the error of one rounding. (float16's are scaled by powers
-    of two before, so that small weights and cotangents keep their digits.)
+    gradient likewise: out has 1.2 times, dq, dk and dv 1.4 times the error of one rounding. (float16's are scaled by
+    powers of two before, so that small weights and cotangents keep their digits.)
 
     Differentiable in q, k, v and table. The gradient keeps q, k, v, out and two float32 a query and
     head; for 16-bit types past 128 queries or keys also what out lost to rounding, as float16."""
